@@ -55,7 +55,10 @@ enum {
 
 enum { VAE_OP_CONV = 1, VAE_OP_CONVT = 2, VAE_OP_BN = 3, VAE_OP_LINEAR = 4,
        VAE_OP_REPARAM = 5, VAE_OP_SLICE0 = 6, VAE_OP_ELBO = 7 };
-enum { VAE_ACT_NONE = 0, VAE_ACT_LEAKY = 1 /* slope in f[0]; 0 => ReLU */, VAE_ACT_SIGMOID = 2 };
+enum { VAE_ACT_NONE = 0, VAE_ACT_LEAKY = 1 /* slope in f[0]; 0 => ReLU */, VAE_ACT_SIGMOID = 2,
+       VAE_ACT_GELU = 3 /* 0.5 p (1 + erf(p / sqrt 2)) */, VAE_ACT_SILU = 4 /* p sigmoid(p) */ /* 3, 4: vae_dense_* only */ };
+/* element types of the sequence-block operators (vae_layer_norm_*, vae_dense_*, vae_gated_scan_*) */
+enum { VAE_T_F32 = 0, VAE_T_BF16 = 1, VAE_T_F16 = 2 };
 enum {
     VAE_F_ACC_DIN = 1,     /* LINEAR/CONV: input grad is accumulated (+=), input has >1 consumer */
     VAE_F_BN_RELU = 2,     /* BN: ReLU fused after normalisation (notebook Conv->BN->ReLU) */
@@ -319,6 +322,51 @@ int vae_randn(float* out, int64_t n, uint64_t* rng, vae_stream_t stream);
  * host-to-device copy in front of train.py:57. */
 int vae_window_gather(const float* series, int C, int64_t T, int L, const int64_t* starts, int B, float* out,
                       vae_stream_t stream);
+
+/* ---- Operators of a sequence block: layer norm, linear with a fused epilogue, gated linear recurrence ------------------
+ * They stand next to BatchNorm, LINEAR and the Conv1d stacks of the 1-D families for models that treat every time step of a
+ * window as a row.  No counterpart in the reference, whose recurrent models are torch LSTMs (Encoders.py:110-147).
+ * dtype = VAE_T_* of the tensors; strides are in elements, rows are contiguous (any alignment, any stride >= the row).  All
+ * sums, statistics and states are fp32.  Workspaces are caller-owned, sized by the *_floats / *_bytes queries (host-only), need no
+ * clearing and hold nothing between calls; calls that may overlap need a workspace each.  Results are bit-identical from run to
+ * run (no float atomics).
+ *
+ * Layer norm over rows of C: y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) with the biased variance.  w, b: type wtype
+ * (VAE_T_F32 or dtype), NULL = 1 / 0.  mean, rstd (rows floats each; both or neither): what the backward pass needs.
+ * Backward: dx, dw, db are optional each; dw and db are the sums over all rows, in wtype; workspace only for those. */
+int vae_layer_norm_forward(const void* x, int64_t ldx, const void* w, const void* b, void* y, int64_t ldy, float* mean,
+                           float* rstd, int64_t rows, int C, float eps, int dtype, int wtype, vae_stream_t stream);
+int64_t vae_layer_norm_workspace_floats(int64_t rows, int C);
+int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
+                            const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* workspace, int64_t rows, int C,
+                            int dtype, int wtype, vae_stream_t stream);
+
+/* Linear layer p = x w^T + bias, y = act(p) + res: x M x K, w N x K, res and y M x N; bias (N), res optional.  act = VAE_ACT_*
+ * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.
+ * Backward: dp = dy act'(p); dx = dp w (M x K, dense), dw = dp^T x (N x K, dense), db = column sums of dp; each optional.  The
+ * residual's gradient is dy itself. */
+int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype);
+int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
+                      void* y, int64_t ldy, void* aux, int M, int N, int K, int act, float slope, int dtype, vae_stream_t stream);
+int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype);
+int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* aux,
+                       void* dx, void* dw, void* db, float* workspace, int M, int N, int K, int act, float slope, int dtype,
+                       vae_stream_t stream);
+
+/* Gated linear recurrence over B sequences of T steps of D features: f = sigmoid(gate), h_t = f h_{t-1} + (1 - f) x_t, y_t = h_t.
+ * x, gate, dy: element (b, t, d) at b*sb + t*st + d; y, dx, dgate: dense B x T x D.  h0, h_last, dh_last, dh0: B x D floats,
+ * optional (absent: zeros).  lengths (B, optional, clamped to 0..T): steps at and behind a sequence's length hold the state; x, gate
+ * and dy are not read there, y, dx and dgate are 0; h_last is the state behind the last step that counts.
+ * kept (vae_gated_scan_kept_floats; NULL when no backward pass follows): states that the backward pass starts its tiles from. */
+int64_t vae_gated_scan_kept_floats(int B, int T, int D);
+int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype);
+int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st,
+                           const float* h0, const int32_t* lengths, void* y, float* h_last, float* kept, float* workspace, int B,
+                           int T, int D, int dtype, vae_stream_t stream);
+int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last, const void* x, int64_t x_sb,
+                            int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st, const float* h0, const int32_t* lengths,
+                            const float* kept, void* dx, void* dgate, float* dh0, float* workspace, int B, int T, int D, int dtype,
+                            vae_stream_t stream);
 
 /* hipGraph capture of an arbitrary sequence of the calls above: begin, issue calls on the
  * returned stream, end -> handle; launch replays on `stream`. */

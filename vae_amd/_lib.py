@@ -13,7 +13,8 @@ LIB_PATH = os.environ.get("VAE_AMD_LIB") or os.path.join(_HERE, "csrc", "libvae_
 
 # enums (include/vae_amd.h)
 OP_CONV, OP_CONVT, OP_BN, OP_LINEAR, OP_REPARAM, OP_SLICE0, OP_ELBO = 1, 2, 3, 4, 5, 6, 7
-ACT_NONE, ACT_LEAKY, ACT_SIGMOID = 0, 1, 2
+ACT_NONE, ACT_LEAKY, ACT_SIGMOID, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4
+T_F32, T_BF16, T_F16 = 0, 1, 2
 F_ACC_DIN, F_BN_RELU, F_KL_GRAD, F_EXT_GRAD, F_BCE, F_IN_RELU, F_FUSED = 1, 2, 4, 8, 16, 32, 64
 F_LOSS_IN_BWD = 128
 F_BN_ACC = 256
@@ -97,6 +98,20 @@ def lib():
     L.vae_adam_step_hyper.argtypes = [vp, vp, vp, vp, i64, vp, vp, vp]
     L.vae_randn.argtypes = [vp, i64, vp, vp]
     L.vae_window_gather.argtypes = [vp, i32, i64, i32, vp, i32, vp, vp]
+    L.vae_layer_norm_forward.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, f32, i32, i32, vp]
+    L.vae_layer_norm_workspace_floats.argtypes = [i64, i32]
+    L.vae_layer_norm_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
+    L.vae_dense_aux_bytes.argtypes = [i64, i64, i32, i32]
+    L.vae_dense_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i32, i32, i32, i32, f32, i32, vp]
+    L.vae_dense_workspace_floats.argtypes = [i64, i64, i64, i32, i32]
+    L.vae_dense_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]
+    L.vae_gated_scan_kept_floats.argtypes = [i32, i32, i32]
+    L.vae_gated_scan_workspace_floats.argtypes = [i32, i32, i32, i32]
+    L.vae_gated_scan_forward.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
+    L.vae_gated_scan_backward.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
+    for name in ("vae_layer_norm_workspace_floats", "vae_dense_aux_bytes", "vae_dense_workspace_floats", "vae_gated_scan_kept_floats",
+                 "vae_gated_scan_workspace_floats"):
+        getattr(L, name).restype = i64
     L.vae_graph_begin.argtypes = [ctypes.POINTER(vp)]
     L.vae_graph_end.argtypes = [ctypes.POINTER(vp)]
     L.vae_graph_launch.argtypes = [vp, vp]
@@ -105,7 +120,8 @@ def lib():
                  "vae_elbo_forward_noalloc", "vae_elbo_backward", "vae_adam_step", "vae_adam_step_hyper", "vae_randn", "vae_window_gather", "vae_graph_begin", "vae_graph_end",
                  "vae_graph_launch", "vae_graph_destroy", "vae_dp_unique_id", "vae_dp_init", "vae_dp_world", "vae_dp_enable",
                  "vae_dp_all_gather_rows", "vae_dp_all_reduce_sum", "vae_dp_shutdown", "vae_run_backward_step",
-                 "vae_dp_set_single_comm", "vae_dp_single_comm", "vae_time_step"):
+                 "vae_dp_set_single_comm", "vae_dp_single_comm", "vae_time_step", "vae_layer_norm_forward", "vae_layer_norm_backward",
+                 "vae_dense_forward", "vae_dense_backward", "vae_gated_scan_forward", "vae_gated_scan_backward"):
         getattr(L, name).restype = i32
     _lib = L
     return L
@@ -118,7 +134,9 @@ EXPORTS = ("vae_seq_scratch_floats", "vae_last_error", "vae_check_device", "vae_
            "vae_elbo_forward_noalloc", "vae_elbo_backward", "vae_adam_step", "vae_adam_step_hyper", "vae_randn", "vae_window_gather", "vae_graph_begin", "vae_graph_end",
            "vae_graph_launch", "vae_graph_destroy", "vae_dp_unique_id", "vae_dp_init", "vae_dp_world", "vae_dp_enable",
            "vae_dp_all_gather_rows", "vae_dp_all_reduce_sum", "vae_dp_shutdown", "vae_run_backward_step",
-           "vae_dp_set_single_comm", "vae_dp_single_comm", "vae_time_step")
+           "vae_dp_set_single_comm", "vae_dp_single_comm", "vae_time_step", "vae_layer_norm_forward", "vae_layer_norm_workspace_floats",
+           "vae_layer_norm_backward", "vae_dense_aux_bytes", "vae_dense_forward", "vae_dense_workspace_floats", "vae_dense_backward",
+           "vae_gated_scan_kept_floats", "vae_gated_scan_workspace_floats", "vae_gated_scan_forward", "vae_gated_scan_backward")
 
 
 _DTYPES = {"f32": 0, "fp32": 0, "float32": 0, "bf16": 1, "bfloat16": 1}

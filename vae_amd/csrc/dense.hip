@@ -1,0 +1,451 @@
+// dense.hip - linear layer with bias, activation and residual in the product's epilogue, forward and backward (vae_dense_*).
+//
+//   p = x W^T + b,  y = act(p) + r        x: M x K, W: N x K (row-major), y, r: M x N
+//   dp = dy act'(p),  dx = dp W,  dW = dp^T x,  db = sum over rows of dp,  dr = dy
+//
+// One product kernel serves all three: C[m][n] = sum_k A(m, k) B(n, k), each operand stored either with k contiguous (x and W in
+// the forward pass, dp in dx) or with its row contiguous (W in dx; dp and x in dW).  Products run on the matrix cores, sums in
+// fp32.
+#include "seqops.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// What the derivative needs of p: one byte that says p > 0 for the leaky ReLU; else p itself, in fp16 where the tensors are bf16
+// (three more bits than their own type: the rounding then adds nothing to what the gradients' own type loses; act' is flat
+// beyond fp16's range, so p is clamped to it) and in fp32 where they are fp16 or fp32.
+enum { AUX_NONE = 0, AUX_U8 = 1, AUX_F16 = 2, AUX_F32 = 4 };
+inline int aux_kind(int act, int dtype) {
+    if (act == VAE_ACT_NONE) return AUX_NONE;
+    if (act == VAE_ACT_LEAKY) return AUX_U8;
+    return dtype == VAE_T_BF16 ? AUX_F16 : AUX_F32;
+}
+
+__device__ __forceinline__ float dense_act(float p, int act, float slope) {
+    switch (act) {
+        case VAE_ACT_LEAKY: return p > 0.f ? p : p * slope;
+        case VAE_ACT_SIGMOID: {
+            float f, i;
+            gate_pair(p, f, i);
+            return f;
+        }
+        case VAE_ACT_GELU: return 0.5f * p * (1.f + erff(p * 0.70710678f));
+        case VAE_ACT_SILU: {
+            float f, i;
+            gate_pair(p, f, i);
+            return p * f;
+        }
+    }
+    return p;
+}
+__device__ __forceinline__ float dense_act_grad(float p, int act) {
+    float f, i;
+    switch (act) {
+        case VAE_ACT_SIGMOID: gate_pair(p, f, i); return f * i;
+        case VAE_ACT_GELU: {
+            if (p > 14.f || p < -14.f) return p > 0.f ? 1.f : 0.f;  // (p exp(-p^2/2) is below fp32's range)
+            return 0.5f * (1.f + erff(p * 0.70710678f)) + p * exp_acc(-0.5f * p * p) * 0.39894228f;
+        }
+        case VAE_ACT_SILU: gate_pair(p, f, i); return f * (1.f + p * i);
+    }
+    return 1.f;
+}
+__device__ __forceinline__ void aux_store(void* aux, int64_t at, float p, int kind) {
+    if (kind == AUX_U8) ((uint8_t*)aux)[at] = p > 0.f ? 1 : 0;
+    else if (kind == AUX_F16) ((f16_t*)aux)[at] = (f16_t)(p > 65504.f ? 65504.f : p < -65504.f ? -65504.f : p);
+    else if (kind == AUX_F32) ((float*)aux)[at] = p;
+}
+__device__ __forceinline__ float aux_grad(const void* aux, int64_t at, int kind, int act, float slope) {
+    if (kind == AUX_U8) return ((const uint8_t*)aux)[at] ? 1.f : slope;
+    return dense_act_grad(kind == AUX_F16 ? (float)((const f16_t*)aux)[at] : ((const float*)aux)[at], act);
+}
+
+struct GemmArgs {
+    const void *a, *b;
+    int64_t lda, ldb;
+    void* c;
+    int64_t ldc;
+    const void *bias, *res;
+    int64_t ldr;
+    void* aux;  // M x N, dense
+    int M, N, K, act, auxk;
+    float slope;
+    float* part;  // split sums: [slices][M][N] instead of c
+    int kslice;
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(const Pack<T, 16 / sizeof(T)>& p, const Pack<T, 16 / sizeof(T)>& q, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mma16<bf16_t>(const Pack<bf16_t, 8>& p, const Pack<bf16_t, 8>& q, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<f16_t>(const Pack<f16_t, 8>& p, const Pack<f16_t, 8>& q, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<float>(const Pack<float, 4>& p, const Pack<float, 4>& q, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p.v[j], q.v[j], c, 0, 0, 0);
+    return c;
+}
+
+// A k-tile of an operand: R rows x 128 bytes of k.  In LDS it lies as it does in memory, with 16-byte pieces permuted so that a
+// fragment's reads spread over the banks:
+//   k contiguous  : [row][8 pieces], piece ^ (row & 7)
+//   row contiguous: [k][R elements], pieces of 32 (16-bit types) or 64 (fp32) bytes permuted by the low bits of k
+constexpr int KB = 128;
+template <typename T>
+constexpr int BK() { return KB / sizeof(T); }
+
+template <typename T, int R, bool RC>
+__device__ __forceinline__ int lds_at(int row, int k) {  // byte offset of the 16-byte piece that holds (row, k)
+    if constexpr (!RC) {
+        const int ch = k * (int)sizeof(T) >> 4;
+        return row * KB + ((ch ^ (row & 7)) << 4);
+    } else if constexpr (sizeof(T) == 2) {
+        int off = row * 2 & ~15;
+        off ^= ((k & 3) | ((k >> 1) & 4)) << 5 & (R * 2 - 1);
+        return k * R * 2 + off;
+    } else {
+        int off = row * 4 & ~15;
+        off ^= ((k >> 2) & 3) << 6;
+        return k * R * 4 + off;
+    }
+}
+
+template <typename T, int R, bool RC, int NT>
+struct Stage {
+    static constexpr int V = 16 / sizeof(T), N = R * 8 / NT;
+    Pack<T, V> r[N];
+    __device__ __forceinline__ void load(const T* p, int64_t ld, int r0, int rows, int k0, int kend, int tid) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = tid + j * NT;
+            if constexpr (!RC) {
+                const int row = r0 + (c >> 3), k = k0 + (c & 7) * V;
+                load_raw<T, V>(r[j], p + (int64_t)row * ld + k, row < rows ? kend - k : 0);
+            } else {
+                const int k = k0 + c / (R / V), row = r0 + c % (R / V) * V;
+                load_raw<T, V>(r[j], p + (int64_t)k * ld + row, k < kend ? rows - row : 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(char* lds, int tid) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = tid + j * NT;
+            const int at = RC ? lds_at<T, R, RC>(c % (R / V) * V, c / (R / V)) : lds_at<T, R, RC>(c >> 3, (c & 7) * V);
+            *reinterpret_cast<uint4*>(lds + at) = __builtin_bit_cast(uint4, r[j]);
+        }
+    }
+};
+
+// The fragment of 16 rows x 64 bytes of k that lane l gives a matrix instruction: row l % 16, k pieces of lane group l / 16.
+template <typename T, int R, bool RC>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> frag(const char* lds, int row0, int ks, int lane) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (!RC) {
+        const int row = row0 + (lane & 15), k = ks * 4 * V + (lane >> 4) * V;
+        return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const uint4*>(lds + lds_at<T, R, RC>(row, k)));
+    } else if constexpr (sizeof(T) == 2) {
+        // a transposing read: 16 lanes read 4 k rows of 16 elements (lane i: k row i / 4, elements 4 (i % 4) ..) and lane i receives
+        // element i of the four
+        Pack<T, V> f;
+        const int i = lane & 15, kq = ks * 32 + (lane >> 4) * 8 + (i >> 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = kq + 4 * h, row = row0 + (i & 3) * 4;
+            const char* at = lds + lds_at<T, R, RC>(row, k) + (row * 2 & 15);
+            const i16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(const_cast<char*>(at)));
+            const Pack<T, 4> q = __builtin_bit_cast(Pack<T, 4>, t);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f.v[4 * h + e] = q.v[e];
+        }
+        return f;
+    } else {
+        Pack<T, V> f;
+        const int row = row0 + (lane & 15);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = ks * 16 + (lane >> 4) * 4 + e;
+            f.v[e] = *reinterpret_cast<const float*>(lds + lds_at<T, R, RC>(row, k) + (row * 4 & 15));
+        }
+        return f;
+    }
+}
+
+// C tile BM x BN by WM x WN waves.  The matrix instruction's first operand is B: a lane then holds four neighbouring columns n of
+// one row m of C.
+template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
+    constexpr int NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+    const int wm = w % WM * (BM / WM), wn = w / WM * (BN / WN);
+    const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
+    Stage<T, BM, ARC, NT> sa;
+    Stage<T, BN, BRC, NT> sb;
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    sa.load((const T*)g.a, g.lda, m0, g.M, k_lo, k_hi, tid);
+    sb.load((const T*)g.b, g.ldb, n0, g.N, k_lo, k_hi, tid);
+    int cur = 0;
+    for (int k0 = k_lo; k0 < k_hi; k0 += BK<T>(), cur ^= 1) {
+        char *pa = lds + cur * (BM + BN) * KB, *pb = pa + BM * KB;
+        sa.put(pa, tid);
+        sb.put(pb, tid);
+        if (k0 + BK<T>() < k_hi) {
+            sa.load((const T*)g.a, g.lda, m0, g.M, k0 + BK<T>(), k_hi, tid);
+            sb.load((const T*)g.b, g.ldb, n0, g.N, k0 + BK<T>(), k_hi, tid);
+        }
+        lds_barrier();  // (two buffers: the writes of the next tile go to the one that no wave reads any more)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            Pack<T, V> fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = frag<T, BM, ARC>(pa, wm + i * 16, ks, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = frag<T, BN, BRC>(pb, wn + j * 16, ks, lane);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+        if (n >= g.N) continue;
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (g.bias != nullptr) load_part<T, 4>(bias, (const T*)g.bias + n, g.N - n);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int m = m0 + wm + i * 16 + (lane & 15);
+            if (m >= g.M) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + bias[e];
+            if (g.part != nullptr) {
+                store_part<float, 4>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, g.N - n);
+                continue;
+            }
+            if (g.aux != nullptr) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < g.N) aux_store(g.aux, (int64_t)m * g.N + n + e, v[e], g.auxk);
+            }
+            float r[4] = {0.f, 0.f, 0.f, 0.f};
+            if (g.res != nullptr) load_part<T, 4>(r, (const T*)g.res + (int64_t)m * g.ldr + n, g.N - n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = dense_act(v[e], g.act, g.slope) + r[e];
+            store_part<T, 4>((T*)g.c + (int64_t)m * g.ldc + n, v, g.N - n);
+        }
+    }
+}
+
+// c = sum of the slices of a split product, in a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_join_k(const float* part, int slices, int64_t n, T* c) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
+#pragma unroll 4
+    for (int k = 0; k < slices; ++k) {
+        load_part<float, 4>(v, part + k * n + i, n - i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+    store_part<T, 4>(c + i, s, n - i);
+}
+
+// dp = dy act'(p), rounded to the type of the products that read it (the matrix cores take their operands so), and the column
+// sums of dp before that rounding: workgroup (x, y) takes 64 columns and every gridDim.y-th block of 32 rows.
+constexpr int ACT_ROWS = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, const void* aux, T* dp, float* part, int M, int N, int act, int auxk,
+                                                    float slope) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (n < N)
+        for (int64_t r0 = (int64_t)blockIdx.y * ACT_ROWS; r0 < M; r0 += (int64_t)gridDim.y * ACT_ROWS)
+            for (int r = w; r < ACT_ROWS && r0 + r < M; r += 4) {
+                const int64_t m = r0 + r;
+                float v = (float)dy[m * ldy + n];
+                if (auxk != AUX_NONE) {
+                    v *= aux_grad(aux, m * N + n, auxk, act, slope);
+                    dp[m * N + n] = (T)v;
+                }
+                s += v;
+            }
+    if (part == nullptr) return;
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
+int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
+    constexpr int bytes = 2 * (BM + BN) * KB;
+    auto* k = gemm_k<T, BM, BN, WM, WN, ARC, BRC>;
+    if (bytes > 65536) {
+        static uint64_t granted = 0;  // per device; a race only repeats the call
+        int dev = 0;
+        VAE_HIP(hipGetDevice(&dev));
+        if (dev < 64 && !(granted >> dev & 1)) {
+            VAE_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            granted |= (uint64_t)1 << dev;
+        }
+    }
+    k<<<dim3((unsigned)ceil_div64(g.N, BN), (unsigned)ceil_div64(g.M, BM), slices), dim3(WM * WN * 64), bytes, s>>>(g);
+    VAE_LAUNCH_CHECK("gemm_k");
+    return VAE_OK;
+}
+
+// Tile of the product: 128 x 128, or 64 x 64 where those give too few workgroups.
+bool gemm_small(int64_t M, int64_t N) { return ceil_div64(M, 128) * ceil_div64(N, 128) < 256; }
+
+// Slices of k of a split product (the weight gradient: few outputs, a long sum): enough workgroups for the chip, at least 8
+// k-tiles each.
+int gemm_slices(int64_t M, int64_t N, int64_t K, int bk, int* kslice) {
+    const int t = gemm_small(M, N) ? 64 : 128;
+    const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), kt = ceil_div64(K, bk);
+    int64_t s = tiles >= 256 ? 1 : ceil_div64(512, tiles);
+    if (s > kt / 8) s = kt / 8;
+    if (s < 1) s = 1;
+    const int64_t per = ceil_div64(kt, s);
+    *kslice = (int)(per * bk);
+    return (int)ceil_div64(kt, per);
+}
+
+template <typename T, bool ARC, bool BRC>
+int gemm(GemmArgs g, float* part, hipStream_t s) {
+    int slices = 1;
+    g.part = nullptr;
+    g.kslice = g.K;
+    if (part != nullptr) {
+        slices = gemm_slices(g.M, g.N, g.K, BK<T>(), &g.kslice);
+        if (slices > 1) g.part = part;
+    }
+    const int rc = gemm_small(g.M, g.N) ? gemm_inst<T, 64, 64, 2, 2, ARC, BRC>(g, slices, s) : gemm_inst<T, 128, 128, 2, 2, ARC, BRC>(g, slices, s);
+    if (rc != VAE_OK || slices == 1) return rc;
+    const int64_t n = (int64_t)g.M * g.N;
+    gemm_join_k<T><<<dim3((unsigned)ceil_div64(n, 1024)), dim3(256), 0, s>>>(part, slices, n, (T*)g.c);
+    VAE_LAUNCH_CHECK("gemm_join_k");
+    return VAE_OK;
+}
+
+int dact_rows(int M) {
+    const int64_t n = ceil_div64(M, ACT_ROWS);
+    return (int)(n < 64 ? n : 64);
+}
+
+struct DenseWs {  // workspace of the backward pass, in floats
+    int64_t dp, split, cols, total;
+};
+DenseWs dense_ws(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+    DenseWs w;
+    const int es = vae_type_size(dtype);
+    const int64_t a = 64;
+    w.dp = 0;
+    w.split = w.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * N * es, 4), a) * a);
+    int ks;
+    const int s = gemm_slices(N, K, M, KB / es, &ks);
+    w.cols = w.split + (s > 1 ? ceil_div64((int64_t)s * N * K, a) * a : 0);
+    w.total = w.cols + 64 * N;
+    return w;
+}
+
+template <typename T>
+int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, int64_t ldw, const void* aux, T* dx, T* dw, T* db, float* ws,
+                     int M, int N, int K, int act, float slope, int dtype, hipStream_t s) {
+    const DenseWs lay = dense_ws(M, N, K, dtype, act);
+    const int auxk = aux_kind(act, dtype);
+    const T* dp = dy;
+    int64_t lddp = lddy;
+    if (auxk != AUX_NONE || db != nullptr) {
+        T* out = (T*)(ws + lay.dp);
+        const int ny = dact_rows(M);
+        float* cols = db != nullptr ? ws + lay.cols : nullptr;
+        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 64), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, cols, M, N, act, auxk, slope);
+        VAE_LAUNCH_CHECK("dense_dact_k");
+        if (auxk != AUX_NONE) dp = out, lddp = N;
+        if (db != nullptr) {
+            gemm_join_k<T><<<dim3((unsigned)ceil_div64(N, 1024)), dim3(256), 0, s>>>(cols, ny, N, db);
+            VAE_LAUNCH_CHECK("gemm_join_k");
+        }
+    }
+    if (dx != nullptr) {
+        GemmArgs g = {};
+        g.a = dp, g.lda = lddp, g.b = w, g.ldb = ldw, g.c = dx, g.ldc = K, g.M = M, g.N = K, g.K = N;
+        if (int rc = gemm<T, false, true>(g, nullptr, s)) return rc;
+    }
+    if (dw != nullptr) {
+        GemmArgs g = {};
+        g.a = dp, g.lda = lddp, g.b = x, g.ldb = ldx, g.c = dw, g.ldc = K, g.M = N, g.N = K, g.K = M;
+        if (int rc = gemm<T, true, true>(g, ws + lay.split, s)) return rc;
+    }
+    return VAE_OK;
+}
+
+int dense_check(const char* what, int64_t M, int64_t N, int64_t K, int act, int dtype) {
+    if (vae_type_size(dtype) == 0) VAE_FAIL(VAE_EINVAL, "%s: type %d (f32, bf16 or f16)", what, dtype);
+    if (act < VAE_ACT_NONE || act > VAE_ACT_SILU) VAE_FAIL(VAE_EINVAL, "%s: activation %d", what, act);
+    if (M < 0 || N < 1 || K < 1 || M > 0x3fffffff || N > 0x3fffffff || K > 0x3fffffff)
+        VAE_FAIL(VAE_EINVAL, "%s: M = %lld, N = %lld, K = %lld", what, (long long)M, (long long)N, (long long)K);
+    return VAE_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype) {
+    return M < 1 || N < 1 ? 0 : M * N * aux_kind(act, dtype);
+}
+
+extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
+                                 void* y, int64_t ldy, void* aux, int M, int N, int K, int act, float slope, int dtype,
+                                 vae_stream_t stream) {
+    if (int rc = dense_check("dense_forward", M, N, K, act, dtype)) return rc;
+    if (M == 0) return VAE_OK;
+    if (x == nullptr || w == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null buffer");
+    if ((M > 1 && (ldx < K || ldy < N || (res != nullptr && ldr < N))) || (N > 1 && ldw < K)) VAE_FAIL(VAE_EINVAL, "dense_forward: a row stride below the row");
+    GemmArgs g = {};
+    g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.c = y, g.ldc = ldy, g.bias = bias, g.res = res, g.ldr = ldr;
+    g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
+    g.aux = g.auxk == AUX_NONE ? nullptr : aux;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == VAE_T_F32) return gemm<float, false, false>(g, nullptr, s);
+    return dtype == VAE_T_BF16 ? gemm<bf16_t, false, false>(g, nullptr, s) : gemm<f16_t, false, false>(g, nullptr, s);
+}
+
+extern "C" int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype) {
+    if (M < 1 || N < 1 || K < 1 || vae_type_size(dtype) == 0) return 0;
+    return dense_ws(M, N, K, dtype, act).total;
+}
+
+extern "C" int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* aux,
+                                  void* dx, void* dw, void* db, float* workspace, int M, int N, int K, int act, float slope, int dtype,
+                                  vae_stream_t stream) {
+    if (int rc = dense_check("dense_backward", M, N, K, act, dtype)) return rc;
+    if (M == 0) VAE_FAIL(VAE_EINVAL, "dense_backward: no rows");
+    if (dy == nullptr || x == nullptr || w == nullptr || workspace == nullptr || (act != VAE_ACT_NONE && aux == nullptr))
+        VAE_FAIL(VAE_EINVAL, "dense_backward: null buffer");
+    if ((M > 1 && (ldx < K || lddy < N)) || (N > 1 && ldw < K)) VAE_FAIL(VAE_EINVAL, "dense_backward: a row stride below the row");
+    hipStream_t s = (hipStream_t)stream;
+#define VAE_DENSE(T) \
+    return dense_backward_t<T>((const T*)dy, lddy, (const T*)x, ldx, (const T*)w, ldw, aux, (T*)dx, (T*)dw, (T*)db, workspace, M, N, K, act, slope, dtype, s)
+    if (dtype == VAE_T_F32) VAE_DENSE(float);
+    if (dtype == VAE_T_BF16) VAE_DENSE(bf16_t);
+    VAE_DENSE(f16_t);
+#undef VAE_DENSE
+}

@@ -1,0 +1,73 @@
+// seqops.h - what the sequence-block operators (norm.hip, dense.hip, gscan.hip) share: element types, loads and stores of
+// any alignment, group sums, the activations in fp32.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+static inline int vae_type_size(int t) { return t == VAE_T_F32 ? 4 : (t == VAE_T_BF16 || t == VAE_T_F16) ? 2 : 0; }
+static inline const char* vae_type_name(int t) { return t == VAE_T_F32 ? "f32" : t == VAE_T_BF16 ? "bf16" : t == VAE_T_F16 ? "f16" : "?"; }
+
+// N elements that start on any multiple of the element's size: gfx950's global loads and stores take such addresses, so
+// rows of odd length move in 16-byte pieces like aligned ones.
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+    T v[N];
+};
+
+// `left` of the N elements at p (the others are 0 and are not read).
+template <typename T, int N>
+__device__ __forceinline__ void load_part(float (&r)[N], const T* p, int64_t left) {
+    if (left >= N) {
+        const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = (float)q.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = i < left ? (float)p[i] : 0.f;
+    }
+}
+// ... as they are in memory, for values that are kept a while before they are used
+template <typename T, int N>
+__device__ __forceinline__ void load_raw(Pack<T, N>& r, const T* p, int64_t left) {
+    if (left >= N) {
+        r = *reinterpret_cast<const Pack<T, N>*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = i < left ? p[i] : (T)0.f;
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_part(T* p, const float (&r)[N], int64_t left) {
+    if (left >= N) {
+        Pack<T, N> q;
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.v[i] = (T)r[i];
+        *reinterpret_cast<Pack<T, N>*>(p) = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) p[i] = (T)r[i];
+    }
+}
+
+// exp(x) with a relative error of about 1e-7 over the whole range: 2^t of t = x log2(e), corrected by what rounding t lost
+// (without the correction |t| 2^-24 enters the result: 1e-6 at |x| = 10).
+__device__ __forceinline__ float exp_acc(float x) {
+    const float t = x * 1.44269504f;
+    const float lost = fmaf(x, 1.44269504f, -t) + x * 1.9259629e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, lost * 0.69314718f, e);
+}
+
+// f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1).  The clamp
+// keeps exp finite; a NaN passes it.
+__device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
+    g = g > 87.f ? 87.f : g;
+    g = g < -87.f ? -87.f : g;
+    const float e = exp_acc(-g);
+    const float r = 1.f / (1.f + e);
+    f = r;
+    i = e * r;
+}

@@ -1,0 +1,299 @@
+"""Operators of a sequence block on the HIP path: layer norm, linear with a fused epilogue, gated linear recurrence.
+
+They stand next to the BatchNorm, Linear and Conv1d ops of the model programs for modules that treat every time step of a
+window as a row: a module built from them trains through `vae_amd.train.train` (autograd path) with `vae_amd.optim.Adam`.
+Each is one or two launches forward and differentiable once.  Tensors are fp32, bf16 or fp16 on an MI355X; sums, statistics and
+states are fp32 (include/vae_amd.h, vae_layer_norm_* / vae_dense_* / vae_gated_scan_*).  Calls run on the current stream of the
+tensors' device, allocate through torch's allocator and can be captured in a graph.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+_TYPES = {torch.float32: L.T_F32, torch.bfloat16: L.T_BF16, torch.float16: L.T_F16}
+_ACTS = {"none": L.ACT_NONE, "leaky": L.ACT_LEAKY, "sigmoid": L.ACT_SIGMOID, "gelu": L.ACT_GELU, "silu": L.ACT_SILU}
+
+
+def _dtype(what, t):
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise L.VaeAmdError(f"{what}: fp32, bf16 or fp16 tensors (got {t.dtype})") from None
+
+
+def _same(what, t, name, shape, dtypes, device):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype not in dtypes:
+        raise L.VaeAmdError(f"{what}: {name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if t.device != device:
+        raise L.VaeAmdError(f"{what}: {name} is on {t.device}, the input on {device}")
+
+
+def _call(fn, name, device, *args):
+    """fn(*args, stream) on the current stream of `device`, whichever device is the current one."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        L.check(rc, name)
+
+
+def _p(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _rows(t, cols):
+    """t as rows of `cols` contiguous elements at one stride: (tensor that owns the memory, rows, stride); copies where the
+    strides are others."""
+    rows = t.numel() // cols if cols else 0
+    if t.is_contiguous():
+        return t, rows, cols
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
+        return t, rows, t.stride(0)
+    if t.dim() > 2 and t.stride(-1) == 1 and t.stride(-2) >= cols and all(
+            t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2)):
+        return t, rows, t.stride(-2)
+    return t.contiguous(), rows, cols
+
+
+def _needs_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+def _norm_forward(x, weight, bias, eps, save):
+    C = x.shape[-1]
+    xr, rows, ld = _rows(x, C)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stat = torch.empty((2, rows), dtype=torch.float32, device=x.device) if save else None
+    w = weight if weight is not None else bias
+    if rows:
+        sp = stat.data_ptr() if save else None
+        _call(L.lib().vae_layer_norm_forward, "vae_layer_norm_forward", x.device, xr.data_ptr(), ld, _p(weight), _p(bias),
+              y.data_ptr(), C, sp, sp + 4 * rows if save else None, rows, C, eps, _TYPES[x.dtype],
+              _TYPES[w.dtype] if w is not None else L.T_F32)
+    return y, xr, stat
+
+
+class _NormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, xr, stat = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(xr, weight, bias, stat)
+        ctx.shape = x.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xr, weight, bias, stat = ctx.saved_tensors
+        C = ctx.shape[-1]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(ctx.shape, dtype=xr.dtype, device=xr.device) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
+        _, rows, ldx = _rows(xr, C)
+        dyr, _, lddy = _rows(dy, C)
+        ws = None
+        if need_w or need_b:
+            ws = torch.empty(L.lib().vae_layer_norm_workspace_floats(rows, C), dtype=torch.float32, device=xr.device)
+        w = weight if weight is not None else bias
+        sp = stat.data_ptr()
+        if C:
+            _call(L.lib().vae_layer_norm_backward, "vae_layer_norm_backward", xr.device, dyr.data_ptr(), lddy, xr.data_ptr(),
+                  ldx, _p(weight), sp, sp + 4 * rows, _p(dx), C, _p(dw), _p(db), _p(ws), rows, C, _TYPES[xr.dtype],
+                  _TYPES[w.dtype] if w is not None else L.T_F32)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, with the biased variance.
+
+    x (..., C); weight, bias (C) or None, fp32 or of x's type (both of one type).  Rows may lie at any stride.  The gradients of
+    weight and bias are sums over all rows in fp32, added in a fixed order."""
+    L.require_device(x)
+    _dtype("layer_norm", x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: input of shape {tuple(x.shape)}")
+    kinds = (torch.float32, x.dtype)
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _same("layer_norm", t, name, x.shape[-1:], kinds, x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise L.VaeAmdError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if _needs_grad(x, weight, bias):
+        return _NormFn.apply(x, weight, bias, float(eps))
+    return _norm_forward(x, weight, bias, float(eps), False)[0]
+
+
+# ---------------------------------------------------------------------------------------------------- linear
+def _linear_forward(x, weight, bias, act, slope, residual, save):
+    N, K = weight.shape
+    xr, M, ldx = _rows(x, K)
+    wr, _, ldw = _rows(weight, K)
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    code = _TYPES[x.dtype]
+    aux = None
+    if M:
+        rr, ldr = None, 0
+        if residual is not None:
+            rr, _, ldr = _rows(residual, N)
+        if save and act != L.ACT_NONE:
+            aux = torch.empty(L.lib().vae_dense_aux_bytes(M, N, act, code), dtype=torch.uint8, device=x.device)
+        _call(L.lib().vae_dense_forward, "vae_dense_forward", x.device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr),
+              ldr, y.data_ptr(), N, _p(aux), M, N, K, act, slope, code)
+    return y, xr, wr, aux
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, slope):
+        y, xr, wr, aux = _linear_forward(x, weight, bias, act, slope, residual, True)
+        ctx.save_for_backward(xr, wr, aux)
+        ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xr, wr, aux = ctx.saved_tensors
+        N, K = wr.shape
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        M = dy.numel() // N
+        dev, dt, code = xr.device, xr.dtype, _TYPES[xr.dtype]
+        alloc = torch.empty if M else torch.zeros
+        dx = alloc(ctx.shape, dtype=dt, device=dev) if need_x else None
+        dw = alloc((N, K), dtype=dt, device=dev) if need_w else None
+        db = alloc((N,), dtype=dt, device=dev) if need_b else None
+        if M and (need_x or need_w or need_b):
+            _, _, ldx = _rows(xr, K)
+            _, _, ldw = _rows(wr, K)
+            dyr, _, lddy = _rows(dy, N)
+            lib = L.lib()
+            ws = torch.empty(lib.vae_dense_workspace_floats(M, N, K, ctx.act, code), dtype=torch.float32, device=dev)
+            _call(lib.vae_dense_backward, "vae_dense_backward", dev, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, wr.data_ptr(), ldw,
+                  _p(aux), _p(dx), _p(dw), _p(db), ws.data_ptr(), M, N, K, ctx.act, ctx.slope, code)
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+def linear(x, weight, bias=None, act="none", slope=0.0, residual=None):
+    """act(x @ weight.T + bias) + residual in one product, everything behind it in the product's epilogue.
+
+    x (..., K), weight (N, K), bias (N) or None, residual (..., N) or None, all of one type (fp32, bf16, fp16).  act: "none", "leaky"
+    (negative side times `slope`; 0: ReLU), "sigmoid", "gelu" (the error function's), "silu".  One row runs as well as many:
+    a served model's single tokens take a form of their own."""
+    L.require_device(x)
+    _dtype("linear", x)
+    if act not in _ACTS:
+        raise ValueError(f"linear: activation {act!r}, expected one of {', '.join(_ACTS)}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
+        raise ValueError(f"linear: input of shape {tuple(x.shape)} with a weight of shape {tuple(weight.shape)}")
+    kinds = (x.dtype,)
+    _same("linear", weight, "weight", weight.shape, kinds, x.device)
+    if bias is not None:
+        _same("linear", bias, "bias", weight.shape[:1], kinds, x.device)
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    if residual is not None:
+        _same("linear", residual, "residual", x.shape[:-1] + weight.shape[:1], kinds, x.device)
+    if _needs_grad(x, weight, bias, residual):
+        return _LinearFn.apply(x, weight, bias, residual, _ACTS[act], float(slope))
+    return _linear_forward(x, weight, bias, _ACTS[act], float(slope), residual, False)[0]
+
+
+# ------------------------------------------------------------------------------------------------ gated scan
+def _steps(t):
+    """t (B, T, D) with contiguous features, as (tensor that owns the memory, sequence stride, step stride)."""
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        t = t.contiguous()
+    return t, t.stride(0), t.stride(1)
+
+
+def _scan_forward(x, gate, h0, lengths, save):
+    B, T, D = x.shape
+    dev = x.device
+    xs, xb, xt = _steps(x)
+    gs, gb, gt = _steps(gate)
+    y = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+    hl = torch.empty((B, D), dtype=torch.float32, device=dev)
+    kept = None
+    lib, code = L.lib(), _TYPES[x.dtype]
+    n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    if save:
+        n = lib.vae_gated_scan_kept_floats(B, T, D)
+        kept = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    _call(lib.vae_gated_scan_forward, "vae_gated_scan_forward", dev, xs.data_ptr(), xb, xt, gs.data_ptr(), gb, gt, _p(h0),
+          _p(lengths), y.data_ptr(), hl.data_ptr(), _p(kept), _p(ws), B, T, D, code)
+    return y, hl, xs, gs, kept
+
+
+class _ScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, lengths):
+        y, hl, xs, gs, kept = _scan_forward(x, gate, h0, lengths, True)
+        ctx.save_for_backward(xs, gs, h0, lengths, kept)
+        ctx.set_materialize_grads(False)
+        return y, hl
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dhl):
+        xs, gs, h0, lengths, kept = ctx.saved_tensors
+        B, T, D = xs.shape
+        dev = xs.device
+        need_x, need_g, need_h = ctx.needs_input_grad[:3]
+        if dy is None and dhl is None:
+            return None, None, None, None
+        dx = torch.empty((B, T, D), dtype=xs.dtype, device=dev) if need_x else None
+        dg = torch.empty((B, T, D), dtype=xs.dtype, device=dev) if need_g else None
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if need_h else None
+        db = dt = 0
+        if dy is not None:
+            dy, db, dt = _steps(dy)
+        if dhl is not None:
+            dhl = dhl.contiguous()
+        lib, code = L.lib(), _TYPES[xs.dtype]
+        n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
+        ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+        _call(lib.vae_gated_scan_backward, "vae_gated_scan_backward", dev, _p(dy), db, dt, _p(dhl), xs.data_ptr(), xs.stride(0),
+              xs.stride(1), gs.data_ptr(), gs.stride(0), gs.stride(1), _p(h0), _p(lengths), _p(kept), _p(dx), _p(dg), _p(dh0),
+              _p(ws), B, T, D, code)
+        return dx, dg, dh0, None
+
+
+def gated_scan(x, gate, h0=None, lengths=None):
+    """h_t = sigmoid(gate_t) h_{t-1} + (1 - sigmoid(gate_t)) x_t over the steps of (B, T, D) windows, every feature by itself.
+
+    Returns (y, h_last): y (B, T, D) holds h_t in x's type, h_last (B, D) the fp32 state behind the last step.  h0 (B, D), fp32: the
+    state before the first step (None: zeros); one step with h0 is how a served model advances.  lengths (B), int32 or int64 on
+    the same device: steps at and behind a sequence's length are padding, whatever they hold; y is 0 there, the state stays.
+    x and gate may be strided views with contiguous features (the halves of one projection)."""
+    L.require_device(x)
+    _dtype("gated_scan", x)
+    if x.dim() != 3:
+        raise ValueError(f"gated_scan: input of shape {tuple(x.shape)}, expected (batch, steps, features)")
+    B, T, D = x.shape
+    _same("gated_scan", gate, "gate", x.shape, (x.dtype,), x.device)
+    if h0 is not None:
+        _same("gated_scan", h0, "h0", (B, D), (torch.float32,), x.device)
+        if not h0.is_contiguous():
+            h0 = h0.contiguous()
+    if lengths is not None:
+        _same("gated_scan", lengths, "lengths", (B,), (torch.int32, torch.int64), x.device)
+        if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+            lengths = lengths.clamp(0, T).to(torch.int32).contiguous()
+    if B == 0 or T == 0 or D == 0:  # no step: the state stays
+        h = h0 if h0 is not None else torch.zeros(B, D, device=x.device)
+        return x * gate, h.clone()
+    if _needs_grad(x, gate, h0):
+        return _ScanFn.apply(x, gate, h0, lengths)
+    return _scan_forward(x, gate, h0, lengths, False)[:2]
