@@ -54,11 +54,6 @@ __device__ __forceinline__ float dense_act_grad(float p, int act) {
     }
     return 1.f;
 }
-__device__ __forceinline__ void aux_store(void* aux, int64_t at, float p, int kind) {
-    if (kind == AUX_U8) ((uint8_t*)aux)[at] = p > 0.f ? 1 : 0;
-    else if (kind == AUX_F16) ((f16_t*)aux)[at] = (f16_t)(p > 65504.f ? 65504.f : p < -65504.f ? -65504.f : p);
-    else if (kind == AUX_F32) ((float*)aux)[at] = p;
-}
 __device__ __forceinline__ float aux_grad(const void* aux, int64_t at, int kind, int act, float slope) {
     if (kind == AUX_U8) return ((const uint8_t*)aux)[at] ? 1.f : slope;
     return dense_act_grad(kind == AUX_F16 ? (float)((const f16_t*)aux)[at] : ((const float*)aux)[at], act);
@@ -180,6 +175,81 @@ __device__ __forceinline__ Pack<T, 16 / sizeof(T)> frag(const char* lds, int row
     }
 }
 
+// 8 neighbouring values of p = x w^T: what an AUX_* buffer keeps of them, left of them in the row
+__device__ __forceinline__ void aux_store8(void* aux, int64_t at, const float (&p)[8], int kind, int left) {
+    if (kind == AUX_U8) {
+        uint8_t* q = (uint8_t*)aux + at;
+        Pack<uint8_t, 8> o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o.v[e] = p[e] > 0.f ? 1 : 0;
+        if (left >= 8) *reinterpret_cast<Pack<uint8_t, 8>*>(q) = o;
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) q[e] = o.v[e];
+    } else if (kind == AUX_F16) {
+        float c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = p[e] > 65504.f ? 65504.f : p[e] < -65504.f ? -65504.f : p[e];
+        store_part<f16_t, 8>((f16_t*)aux + at, c, left);
+    } else if (kind == AUX_F32) {
+        store_part<float, 8>((float*)aux + at, p, left);
+    }
+}
+
+// bias, what the backward pass needs, activation, residual, and the store of 8 neighbouring columns of a row
+template <typename T>
+__device__ __forceinline__ void finish8(const GemmArgs& g, float (&v)[8], int64_t m, int n) {
+    const int left = g.N - n;
+    if (g.part != nullptr) {
+        store_part<float, 8>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, left);
+        return;
+    }
+    float t[8];
+    if (g.bias != nullptr) {
+        load_part<T, 8>(t, (const T*)g.bias + n, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    if (g.aux != nullptr) aux_store8(g.aux, m * g.N + n, v, g.auxk, left);
+    if (g.act != VAE_ACT_NONE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = dense_act(v[e], g.act, g.slope);
+    }
+    if (g.res != nullptr) {
+        load_part<T, 8>(t, (const T*)g.res + m * g.ldr + n, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    store_part<T, 8>((T*)g.c + m * g.ldc + n, v, left);
+}
+
+// The epilogue of a wave's share of C: acc[i][j][e] is row i * 16 + lane % 16, column j * 16 + lane / 16 * 4 + e.  Two rows of
+// fragments at a time go through LDS (sm: the wave's own part of the tile buffers, free by now), so that lanes hold 8 neighbouring
+// columns and a row leaves in whole lines.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)[FM][FN], int m0, int n0, int lane, float* sm) {
+    constexpr int LD = FN * 16 + 4, LPR = FN * 2, RPP = 64 / LPR;  // floats of a row in LDS, lanes a row, rows a pass
+#pragma unroll
+    for (int i = 0; i < FM; i += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(sm + (h * 16 + (lane & 15)) * LD + j * 16 + (lane >> 4) * 4) = acc[i + h][j];
+        // (one wave writes and reads: LDS keeps its order)
+        const int n = n0 + lane % LPR * 8;
+#pragma unroll 1
+        for (int r = lane / LPR; r < 32; r += RPP) {
+            const int m = m0 + i * 16 + r;
+            if (m >= g.M || n >= g.N) continue;
+            const float* q = sm + r * LD + lane % LPR * 8;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            finish8<T>(g, v, m, n);
+        }
+    }
+}
+
 // C tile BM x BN by WM x WN waves.  The matrix instruction's first operand is B: a lane then holds four neighbouring columns n of
 // one row m of C.
 template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
@@ -222,35 +292,130 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
                 for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
         }
     }
+    __syncthreads();
+    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
+}
+
+// ---- The large products -----------------------------------------------------------------------------------------------
+// Operands whose rows are whole 16-byte pieces go from memory to LDS without passing registers (buffer loads with an LDS
+// destination: 64 lanes x 16 bytes land side by side, so the permutation of lds_at is applied to the addresses they come from).
+// What lies outside the operand is bounds-checked by the buffer descriptor and arrives as 0.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
+    // no register is written and the addresses are read when the instruction issues; the caller waits (vmcnt) before the
+    // barrier behind which the tile is read
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rsrc));
+}
+
+template <typename T, int R, bool RC, int NT>
+struct Dma {
+    static constexpr int V = 16 / sizeof(T), N = R * 8 / NT, PER_ROW = RC ? R / V : 8;  // N instructions a wave; 16-byte pieces of a stored row
+    uint32_t voff[N];
+    int kk[N];  // KC: first k of the lane's piece (tail check)
+    uint64_t base;
+    int64_t ld;
+    int rows;
+    uint32_t lds0;
+    __device__ __forceinline__ void init(const T* p, int64_t ld_, int r0, int R_total, int tid) {
+        const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        ld = ld_;
+        rows = R_total - r0 < R ? R_total - r0 : R;
+        base = (uint64_t)(p + (RC ? (int64_t)r0 : (int64_t)r0 * ld));
+        lds0 = w * N * 1024;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-        if (n >= g.N) continue;
-        float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (g.bias != nullptr) load_part<T, 4>(bias, (const T*)g.bias + n, g.N - n);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const int m = m0 + wm + i * 16 + (lane & 15);
-            if (m >= g.M) continue;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + bias[e];
-            if (g.part != nullptr) {
-                store_part<float, 4>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, g.N - n);
-                continue;
-            }
-            if (g.aux != nullptr) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < g.N) aux_store(g.aux, (int64_t)m * g.N + n + e, v[e], g.auxk);
-            }
-            float r[4] = {0.f, 0.f, 0.f, 0.f};
-            if (g.res != nullptr) load_part<T, 4>(r, (const T*)g.res + (int64_t)m * g.ldr + n, g.N - n);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = dense_act(v[e], g.act, g.slope) + r[e];
-            store_part<T, 4>((T*)g.c + (int64_t)m * g.ldc + n, v, g.N - n);
+        for (int j = 0; j < N; ++j) {
+            const int piece = (w * N + j) * 64 + lane;  // in the tile as it lies in LDS
+            const int line = piece / PER_ROW, ph = (piece % PER_ROW) * 16;
+            int lo;  // byte in the stored row that belongs there (lds_at is its own inverse within a row)
+            if constexpr (!RC) lo = lds_at<T, R, false>(line, ph / (int)sizeof(T)) - line * KB;
+            else lo = lds_at<T, R, true>(ph / (int)sizeof(T), line) - line * R * (int)sizeof(T);
+            kk[j] = lo / (int)sizeof(T);
+            voff[j] = (uint32_t)(line * ld * (int64_t)sizeof(T)) + lo;
+            if (RC && kk[j] >= rows) voff[j] = 0x80000000u;
         }
     }
+    // issue instructions [j0, j1) of the tile at k0 into the LDS buffer at `lds`
+    __device__ __forceinline__ void issue(int j, uint32_t lds, int k0, int kend) const {
+        const uint64_t at = base + (RC ? (uint64_t)((int64_t)k0 * ld) : (uint64_t)k0) * sizeof(T);
+        const int64_t left = kend - k0;
+        const int64_t bytes = RC ? ((left - 1) * ld + rows) * (int64_t)sizeof(T) : ((rows - 1) * ld + left) * (int64_t)sizeof(T);
+        i32x4 d;
+        d.x = (int)(uint32_t)at;
+        d.y = (int)((uint32_t)(at >> 32) & 0xffff);
+        d.z = left <= 0 ? 0 : (int)(bytes < 0x7fffffff ? bytes : 0x7fffffff);
+        d.w = 0x00020000;
+        uint32_t o = voff[j];
+        if (!RC && left < BK<T>() && kk[j] >= left) o = 0x80000000u;
+        dma16(d, lds + lds0 + j * 1024, o);
+    }
+};
+
+// One wave a SIMD with a 128 x 128 (BM = BN = 256) share of C in its accumulators: a fragment read from LDS then serves eight
+// matrix instructions, and LDS moves 64 + 64 bytes for 1024 cycles of matrix work (with 64 x 128 shares it would be the bound).
+// The k-loop runs in two phases of half a tile.  While the matrix cores work on one half, the fragments of the next half are
+// read; between the phases of a tile one barrier says at once that the next tile has landed and that this one has been read,
+// so its buffer is filled again from there on: a load has a whole tile's time to arrive.
+template <typename T, int BM, int BN, bool ARC, bool BRC>
+__global__ __launch_bounds__(256, 1) void gemm_dma_k(const GemmArgs g) {
+    constexpr int NT = 256, V = 16 / sizeof(T), FM = BM / 32, FN = BN / 32, TILE = (BM + BN) * KB;
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+    const int wm = (w & 1) * (BM / 2), wn = (w >> 1) * (BN / 2);
+    const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
+    const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    Dma<T, BM, ARC, NT> da;
+    Dma<T, BN, BRC, NT> db;
+    da.init((const T*)g.a, g.lda, m0, g.M, tid);
+    db.init((const T*)g.b, g.ldb, n0, g.N, tid);
+    constexpr int DN = Dma<T, BM, ARC, NT>::N;
+    static_assert(BM == BN, "one number of instructions for both operands");
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < DN; ++j) da.issue(j, lbase, k_lo, k_hi), db.issue(j, lbase + BM * KB, k_lo, k_hi);
+#pragma unroll
+    for (int j = 0; j < DN; ++j) da.issue(j, lbase + TILE, k_lo + BK<T>(), k_hi), db.issue(j, lbase + TILE + BM * KB, k_lo + BK<T>(), k_hi);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * DN) : "memory");
+    Pack<T, V> fa[2][FM], fb[2][FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[0][j] = frag<T, BN, BRC>(lds + BM * KB, wn + j * 16, 0, lane);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[0][i] = frag<T, BM, ARC>(lds, wm + i * 16, 0, lane);
+    int cur = 0;
+    for (int k0 = k_lo; k0 < k_hi; k0 += BK<T>(), cur ^= 1) {
+        const char *pa = lds + cur * TILE, *pb = pa + BM * KB;
+        const char *qa = lds + (cur ^ 1) * TILE, *qb = qa + BM * KB;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            fb[1][i] = frag<T, BN, BRC>(pb, wn + i * 16, 1, lane);
+            fa[1][i] = frag<T, BM, ARC>(pa, wm + i * 16, 1, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[0][j], fa[0][i], acc[i][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const uint32_t fill = lbase + cur * TILE;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            fb[0][i] = frag<T, BN, BRC>(qb, wn + i * 16, 0, lane);
+            fa[0][i] = frag<T, BM, ARC>(qa, wm + i * 16, 0, lane);
+            if (i < DN) da.issue(i, fill, k0 + 2 * BK<T>(), k_hi), db.issue(i, fill + BM * KB, k0 + 2 * BK<T>(), k_hi);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[1][j], fa[1][i], acc[i][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    static_assert(DN <= FM, "the loads of a tile are spread over one phase");
+    // (the loads behind the last tile bring nothing, but they must have ended before LDS is used for something else)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
 
 // c = sum of the slices of a split product, in a fixed order
@@ -294,10 +459,13 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
     if (w == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
+template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC, bool DMA>
 int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     constexpr int bytes = 2 * (BM + BN) * KB;
-    auto* k = gemm_k<T, BM, BN, WM, WN, ARC, BRC>;
+    static_assert(WM * WN * 32 * (BN / WN + 4) * 4 <= bytes, "the epilogue's LDS");
+    void (*k)(const GemmArgs);
+    if constexpr (DMA) k = gemm_dma_k<T, BM, BN, ARC, BRC>;
+    else k = gemm_k<T, BM, BN, WM, WN, ARC, BRC>;
     if (bytes > 65536) {
         static uint64_t granted = 0;  // per device; a race only repeats the call
         int dev = 0;
@@ -314,6 +482,17 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
 
 // Tile of the product: 128 x 128, or 64 x 64 where those give too few workgroups.
 bool gemm_small(int64_t M, int64_t N) { return ceil_div64(M, 128) * ceil_div64(N, 128) < 256; }
+
+bool gemm_large(int64_t M, int64_t N) { return ceil_div64(M, 256) * ceil_div64(N, 256) >= 192; }
+
+// Can the operands go to LDS directly: rows that start and end on 16 bytes, a tile's rows within 31 bits of offset.
+template <typename T>
+bool whole_pieces(const GemmArgs& g, bool arc, bool brc) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t most = (int64_t)0x7fffffff / (256 * sizeof(T)) - 64;
+    return ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.lda % V == 0 && g.ldb % V == 0 && (arc ? g.M : g.K) % V == 0 &&
+           (brc ? g.N : g.K) % V == 0 && g.lda < most && g.ldb < most;
+}
 
 // Slices of k of a split product (the weight gradient: few outputs, a long sum): enough workgroups for the chip, at least 8
 // k-tiles each.
@@ -337,7 +516,10 @@ int gemm(GemmArgs g, float* part, hipStream_t s) {
         slices = gemm_slices(g.M, g.N, g.K, BK<T>(), &g.kslice);
         if (slices > 1) g.part = part;
     }
-    const int rc = gemm_small(g.M, g.N) ? gemm_inst<T, 64, 64, 2, 2, ARC, BRC>(g, slices, s) : gemm_inst<T, 128, 128, 2, 2, ARC, BRC>(g, slices, s);
+    int rc;
+    if (gemm_small(g.M, g.N)) rc = gemm_inst<T, 64, 64, 2, 2, ARC, BRC, false>(g, slices, s);
+    else if (gemm_large(g.M, g.N) && whole_pieces<T>(g, ARC, BRC)) rc = gemm_inst<T, 256, 256, 2, 2, ARC, BRC, true>(g, slices, s);
+    else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, false>(g, slices, s);
     if (rc != VAE_OK || slices == 1) return rc;
     const int64_t n = (int64_t)g.M * g.N;
     gemm_join_k<T><<<dim3((unsigned)ceil_div64(n, 1024)), dim3(256), 0, s>>>(part, slices, n, (T*)g.c);
