@@ -54,11 +54,6 @@ __device__ __forceinline__ float dense_act_grad(float p, int act) {
     }
     return 1.f;
 }
-__device__ __forceinline__ float aux_grad(const void* aux, int64_t at, int kind, int act, float slope) {
-    if (kind == AUX_U8) return ((const uint8_t*)aux)[at] ? 1.f : slope;
-    return dense_act_grad(kind == AUX_F16 ? (float)((const f16_t*)aux)[at] : ((const float*)aux)[at], act);
-}
-
 struct GemmArgs {
     const void *a, *b;
     int64_t lda, ldb;
@@ -92,17 +87,17 @@ __device__ __forceinline__ f32x4 mma16<float>(const Pack<float, 4>& p, const Pac
 
 // A k-tile of an operand: R rows x 128 bytes of k.  In LDS it lies as it does in memory, with 16-byte pieces permuted so that a
 // fragment's reads spread over the banks:
-//   k contiguous  : [row][8 pieces], piece ^ (row & 7)
+//   k contiguous  : [row][8 pieces], piece ^ (row & 7); in half tiles [row][4 pieces], piece ^ (row / 2 & 3)
 //   row contiguous: [k][R elements], pieces of 32 (16-bit types) or 64 (fp32) bytes permuted by the low bits of k
 constexpr int KB = 128;
 template <typename T>
 constexpr int BK() { return KB / sizeof(T); }
 
-template <typename T, int R, bool RC>
+template <typename T, int R, bool RC, int KBYTES = KB>
 __device__ __forceinline__ int lds_at(int row, int k) {  // byte offset of the 16-byte piece that holds (row, k)
     if constexpr (!RC) {
         const int ch = k * (int)sizeof(T) >> 4;
-        return row * KB + ((ch ^ (row & 7)) << 4);
+        return row * KBYTES + ((ch ^ (KBYTES == 128 ? row & 7 : (row >> 1) & 3)) << 4);
     } else if constexpr (sizeof(T) == 2) {
         int off = row * 2 & ~15;
         off ^= ((k & 3) | ((k >> 1) & 4)) << 5 & (R * 2 - 1);
@@ -141,22 +136,22 @@ struct Stage {
     }
 };
 
-// The fragment of 16 rows x 64 bytes of k that lane l gives a matrix instruction: row l % 16, k pieces of lane group l / 16.
-template <typename T, int R, bool RC>
+// The fragment of 16 rows x 64 bytes of k that lane l gives a matrix instruction: row l % 16, the l / 16-th of 4 pieces of 16 bytes.
+// ks counts fragments along k.
+template <typename T, int R, bool RC, int KBYTES = KB>
 __device__ __forceinline__ Pack<T, 16 / sizeof(T)> frag(const char* lds, int row0, int ks, int lane) {
     constexpr int V = 16 / sizeof(T);
+    const int kq = (ks * 4 + (lane >> 4)) * V;
     if constexpr (!RC) {
-        const int row = row0 + (lane & 15), k = ks * 4 * V + (lane >> 4) * V;
-        return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const uint4*>(lds + lds_at<T, R, RC>(row, k)));
+        return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const uint4*>(lds + lds_at<T, R, RC, KBYTES>(row0 + (lane & 15), kq)));
     } else if constexpr (sizeof(T) == 2) {
         // a transposing read: 16 lanes read 4 k rows of 16 elements (lane i: k row i / 4, elements 4 (i % 4) ..) and lane i receives
         // element i of the four
         Pack<T, V> f;
-        const int i = lane & 15, kq = ks * 32 + (lane >> 4) * 8 + (i >> 2);
+        const int i = lane & 15, row = row0 + (i & 3) * 4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int k = kq + 4 * h, row = row0 + (i & 3) * 4;
-            const char* at = lds + lds_at<T, R, RC>(row, k) + (row * 2 & 15);
+            const char* at = lds + lds_at<T, R, RC, KBYTES>(row, kq + (i >> 2) + 4 * h) + (row * 2 & 15);
             const i16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(const_cast<char*>(at)));
             const Pack<T, 4> q = __builtin_bit_cast(Pack<T, 4>, t);
 #pragma unroll
@@ -167,10 +162,7 @@ __device__ __forceinline__ Pack<T, 16 / sizeof(T)> frag(const char* lds, int row
         Pack<T, V> f;
         const int row = row0 + (lane & 15);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = ks * 16 + (lane >> 4) * 4 + e;
-            f.v[e] = *reinterpret_cast<const float*>(lds + lds_at<T, R, RC>(row, k) + (row * 4 & 15));
-        }
+        for (int e = 0; e < 4; ++e) f.v[e] = *reinterpret_cast<const float*>(lds + lds_at<T, R, RC, KBYTES>(row, kq + e) + (row * 4 & 15));
         return f;
     }
 }
@@ -250,6 +242,18 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
     }
 }
 
+// The tile of a workgroup.  Workgroups go round the 8 XCDs in turn, each with an L2 of its own: an XCD takes a contiguous share of
+// the tiles, in blocks 8 tiles of m high, so that its 32 CUs read 8 + 4 panels of the operands and not 32 + 32.
+__device__ __forceinline__ void tile_of(int M, int N, int BM, int BN, int& m, int& n) {
+    const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, tiles = tm * tn;
+    const int x = blockIdx.x & 7, q = tiles >> 3, r = tiles & 7;
+    const int o = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
+    const int per = 8 * tn, grp = o / per, in = o - grp * per;
+    const int h = tm - grp * 8 < 8 ? tm - grp * 8 : 8;
+    n = in / h;
+    m = grp * 8 + (in - n * h);
+}
+
 // C tile BM x BN by WM x WN waves.  The matrix instruction's first operand is B: a lane then holds four neighbouring columns n of
 // one row m of C.
 template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
@@ -257,7 +261,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
     constexpr int NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+    int m0, n0;
+    tile_of(g.M, g.N, BM, BN, m0, n0);
+    m0 *= BM, n0 *= BN;
     const int wm = w % WM * (BM / WM), wn = w / WM * (BN / WN);
     const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
     Stage<T, BM, ARC, NT> sa;
@@ -308,14 +314,17 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t lds_addr, uint32_t vo
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rsrc));
 }
 
+constexpr int HB = 64;  // bytes of k in a half tile
+template <typename T>
+constexpr int HK() { return HB / sizeof(T); }
+
 template <typename T, int R, bool RC, int NT>
 struct Dma {
-    static constexpr int V = 16 / sizeof(T), N = R * 8 / NT, PER_ROW = RC ? R / V : 8;  // N instructions a wave; 16-byte pieces of a stored row
+    static constexpr int V = 16 / sizeof(T), N = R * 4 / NT, PER_ROW = RC ? R / V : 4;  // N instructions a wave; 16-byte pieces of a stored row
     uint32_t voff[N];
-    int kk[N];  // KC: first k of the lane's piece (tail check)
     uint64_t base;
     int64_t ld;
-    int rows;
+    int rows, kk;  // kk (k contiguous): first k of the lane's pieces
     uint32_t lds0;
     __device__ __forceinline__ void init(const T* p, int64_t ld_, int r0, int R_total, int tid) {
         const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -323,45 +332,49 @@ struct Dma {
         rows = R_total - r0 < R ? R_total - r0 : R;
         base = (uint64_t)(p + (RC ? (int64_t)r0 : (int64_t)r0 * ld));
         lds0 = w * N * 1024;
+        kk = (((lane & 3) ^ (lane >> 3 & 3)) << 4) / (int)sizeof(T);  // (16 rows an instruction: the same for all of them)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int piece = (w * N + j) * 64 + lane;  // in the tile as it lies in LDS
+            const int piece = (w * N + j) * 64 + lane;  // in the half tile as it lies in LDS
             const int line = piece / PER_ROW, ph = (piece % PER_ROW) * 16;
-            int lo;  // byte in the stored row that belongs there (lds_at is its own inverse within a row)
-            if constexpr (!RC) lo = lds_at<T, R, false>(line, ph / (int)sizeof(T)) - line * KB;
-            else lo = lds_at<T, R, true>(ph / (int)sizeof(T), line) - line * R * (int)sizeof(T);
-            kk[j] = lo / (int)sizeof(T);
+            // byte in the stored row that belongs there (lds_at is its own inverse within a row)
+            const int lo = RC ? lds_at<T, R, true, HB>(ph / (int)sizeof(T), line) - line * R * (int)sizeof(T) : kk * (int)sizeof(T);
             voff[j] = (uint32_t)(line * ld * (int64_t)sizeof(T)) + lo;
-            if (RC && kk[j] >= rows) voff[j] = 0x80000000u;
+            if (RC && lo / (int)sizeof(T) >= rows) voff[j] = 0x80000000u;
         }
     }
-    // issue instructions [j0, j1) of the tile at k0 into the LDS buffer at `lds`
-    __device__ __forceinline__ void issue(int j, uint32_t lds, int k0, int kend) const {
-        const uint64_t at = base + (RC ? (uint64_t)((int64_t)k0 * ld) : (uint64_t)k0) * sizeof(T);
-        const int64_t left = kend - k0;
-        const int64_t bytes = RC ? ((left - 1) * ld + rows) * (int64_t)sizeof(T) : ((rows - 1) * ld + left) * (int64_t)sizeof(T);
+    // the descriptor of the half tile at k0: what it bounds arrives, the rest is 0.  (32-bit sizes: 256 rows lie within 31 bits)
+    __device__ __forceinline__ i32x4 at(int k0, int kend) const {
+        const uint64_t p = base + (RC ? (uint64_t)((int64_t)k0 * ld) : (uint64_t)k0) * sizeof(T);
+        const int left = kend - k0 < HK<T>() ? kend - k0 : HK<T>();
+        const int pitch = (int)ld * (int)sizeof(T);
         i32x4 d;
-        d.x = (int)(uint32_t)at;
-        d.y = (int)((uint32_t)(at >> 32) & 0xffff);
-        d.z = left <= 0 ? 0 : (int)(bytes < 0x7fffffff ? bytes : 0x7fffffff);
+        d.x = (int)(uint32_t)p;
+        d.y = (int)((uint32_t)(p >> 32) & 0xffff);
+        d.z = left <= 0 ? 0 : RC ? (left - 1) * pitch + rows * (int)sizeof(T) : (rows - 1) * pitch + left * (int)sizeof(T);
         d.w = 0x00020000;
-        uint32_t o = voff[j];
-        if (!RC && left < BK<T>() && kk[j] >= left) o = 0x80000000u;
-        dma16(d, lds + lds0 + j * 1024, o);
+        return d;
+    }
+    __device__ __forceinline__ void issue(int j, i32x4 d, uint32_t lds, bool tail) const {
+        dma16(d, lds + lds0 + j * 1024, !RC && tail ? 0x80000000u : voff[j]);
     }
 };
 
-// One wave a SIMD with a 128 x 128 (BM = BN = 256) share of C in its accumulators: a fragment read from LDS then serves eight
-// matrix instructions, and LDS moves 64 + 64 bytes for 1024 cycles of matrix work (with 64 x 128 shares it would be the bound).
-// The k-loop runs in two phases of half a tile.  While the matrix cores work on one half, the fragments of the next half are
-// read; between the phases of a tile one barrier says at once that the next tile has landed and that this one has been read,
-// so its buffer is filled again from there on: a load has a whole tile's time to arrive.
+// One wave a SIMD with a 128 x 128 (BM = BN = 256) share of C in its accumulators: a fragment read from LDS then serves eight matrix
+// instructions, and LDS moves 96 bytes a cycle (with 64 x 128 shares it would be 128, all that it can).  (BM = BN = 128: two workgroups
+// a CU, for products with too few tiles of 256.)  The k-loop runs in phases of 64 bytes of k.  In phase h the matrix cores work on the fragments of half tile h, the fragments of h + 1 are read, and the loads
+// of h + 4 are issued into the slot of a ring of four that h has left: a load has two phases and more to arrive.  One barrier a phase
+// says that h + 2 has landed for every wave and that h + 1 has been read by every wave.  Reads and loads stand between the matrix
+// instructions, one at a time, where their issue costs nothing.
 template <typename T, int BM, int BN, bool ARC, bool BRC>
-__global__ __launch_bounds__(256, 1) void gemm_dma_k(const GemmArgs g) {
-    constexpr int NT = 256, V = 16 / sizeof(T), FM = BM / 32, FN = BN / 32, TILE = (BM + BN) * KB;
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmArgs g) {
+    constexpr int NT = 256, V = 16 / sizeof(T), FM = BM / 32, FN = BN / 32, SLOT = (BM + BN) * HB;
+    constexpr int RPR = (FM + FN + FM - 3) / (FM - 2);  // fragments read a row of matrix instructions
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+    int m0, n0;
+    tile_of(g.M, g.N, BM, BN, m0, n0);
+    m0 *= BM, n0 *= BN;
     const int wm = (w & 1) * (BM / 2), wn = (w >> 1) * (BN / 2);
     const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
     const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -377,44 +390,61 @@ __global__ __launch_bounds__(256, 1) void gemm_dma_k(const GemmArgs g) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < DN; ++j) da.issue(j, lbase, k_lo, k_hi), db.issue(j, lbase + BM * KB, k_lo, k_hi);
+    for (int h = 0; h < 4; ++h) {
+        const int k = k_lo + h * HK<T>();
+        const i32x4 a = da.at(k, k_hi), b = db.at(k, k_hi);
 #pragma unroll
-    for (int j = 0; j < DN; ++j) da.issue(j, lbase + TILE, k_lo + BK<T>(), k_hi), db.issue(j, lbase + TILE + BM * KB, k_lo + BK<T>(), k_hi);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * DN) : "memory");
-    Pack<T, V> fa[2][FM], fb[2][FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) fb[0][j] = frag<T, BN, BRC>(lds + BM * KB, wn + j * 16, 0, lane);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) fa[0][i] = frag<T, BM, ARC>(lds, wm + i * 16, 0, lane);
-    int cur = 0;
-    for (int k0 = k_lo; k0 < k_hi; k0 += BK<T>(), cur ^= 1) {
-        const char *pa = lds + cur * TILE, *pb = pa + BM * KB;
-        const char *qa = lds + (cur ^ 1) * TILE, *qb = qa + BM * KB;
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-            fb[1][i] = frag<T, BN, BRC>(pb, wn + i * 16, 1, lane);
-            fa[1][i] = frag<T, BM, ARC>(pa, wm + i * 16, 1, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[0][j], fa[0][i], acc[i][j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const uint32_t fill = lbase + cur * TILE;
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-            fb[0][i] = frag<T, BN, BRC>(qb, wn + i * 16, 0, lane);
-            fa[0][i] = frag<T, BM, ARC>(qa, wm + i * 16, 0, lane);
-            if (i < DN) da.issue(i, fill, k0 + 2 * BK<T>(), k_hi), db.issue(i, fill + BM * KB, k0 + 2 * BK<T>(), k_hi);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[1][j], fa[1][i], acc[i][j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < DN; ++j) da.issue(j, a, lbase + h * SLOT, da.kk >= k_hi - k), db.issue(j, b, lbase + h * SLOT + BM * HB, db.kk >= k_hi - k);
     }
-    static_assert(DN <= FM, "the loads of a tile are spread over one phase");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * DN) : "memory");  // the first two have landed
+    Pack<T, V> fa[2][FM], fb[2][FN];                                              // [phase's parity]
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[0][j] = frag<T, BN, BRC, HB>(lds + BM * HB, wn + j * 16, 0, lane);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[0][i] = frag<T, BM, ARC, HB>(lds, wm + i * 16, 0, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // slot 0 has been read
+    uint32_t slot = 0;  // of the half tile in work
+    i32x4 a = da.at(k_lo + 4 * HK<T>(), k_hi), b = db.at(k_lo + 4 * HK<T>(), k_hi);  // of the half tile that is loaded next
+    bool tail = da.kk >= k_hi - (k_lo + 4 * HK<T>());
+    for (int k0 = k_lo; k0 < k_hi; k0 += 2 * HK<T>()) {
+#pragma unroll
+        for (int par = 0; par < 2; ++par) {
+            const uint32_t fill = lbase + slot * SLOT;
+            slot = (slot + 1) & 3;
+            const char *pa = lds + slot * SLOT, *pb = pa + BM * HB;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {  // a row of fragments: FN matrix instructions and a share of the reads and loads
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    acc[i][j] = mma16<T>(fb[par][j], fa[par][i], acc[i][j]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j == FN - 1) {
+                        if (i < DN) da.issue(i, a, fill, tail);
+                        else if (i < 2 * DN) db.issue(i - DN, b, fill + BM * HB, tail);
+                    }
+#pragma unroll
+                    for (int r = 0; r < RPR; ++r) {  // (the last two rows' time is left for the reads to end)
+                        const int f = i * RPR + r;   // B's fragments, then A's
+                        if (r * FN / RPR != j || i >= FM - 2 || f >= FN + FM) continue;
+                        if (f < FN) fb[par ^ 1][f] = frag<T, BN, BRC, HB>(pb, wn + f * 16, 0, lane);
+                        else fa[par ^ 1][f - FN] = frag<T, BM, ARC, HB>(pa, wm + (f - FN) * 16, 0, lane);
+                    }
+                }
+                if (i == FM - 1) {  // (here the scalar unit is free; at a phase's head the matrix cores would wait for it)
+                    int k5 = k0 + (5 + par) * HK<T>();
+                    asm volatile("" : "+s"(k5));  // (nothing of it moves up)
+                    a = da.at(k5, k_hi), b = db.at(k5, k_hi);
+                    tail = da.kk >= k_hi - k5;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * DN) : "memory");
+        }
+    }
+    static_assert(2 * DN <= FM && RPR <= FN, "a phase holds the loads and the reads");
     // (the loads behind the last tile bring nothing, but they must have ended before LDS is used for something else)
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
 
@@ -433,30 +463,50 @@ __global__ __launch_bounds__(256) void gemm_join_k(const float* part, int slices
     store_part<T, 4>(c + i, s, n - i);
 }
 
-// dp = dy act'(p), rounded to the type of the products that read it (the matrix cores take their operands so), and the column
-// sums of dp before that rounding: workgroup (x, y) takes 64 columns and every gridDim.y-th block of 32 rows.
-constexpr int ACT_ROWS = 32;
+// dp = dy act'(p), rounded to the type of the products that read it (the matrix cores take their operands so), and the column sums
+// of dp before that rounding.  Bound: bytes (dy and p read, dp written).  A workgroup takes 256 columns, 8 neighbouring ones a
+// lane, 8 rows at a time, and every gridDim.y-th block of rows; its sums stay in registers until the end.
+constexpr int ACT_ROWS = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, const void* aux, T* dp, float* part, int M, int N, int act, int auxk,
                                                     float slope) {
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
-    float s = 0.f;
-    if (n < N)
-        for (int64_t r0 = (int64_t)blockIdx.y * ACT_ROWS; r0 < M; r0 += (int64_t)gridDim.y * ACT_ROWS)
-            for (int r = w; r < ACT_ROWS && r0 + r < M; r += 4) {
-                const int64_t m = r0 + r;
-                float v = (float)dy[m * ldy + n];
-                if (auxk != AUX_NONE) {
-                    v *= aux_grad(aux, m * N + n, auxk, act, slope);
-                    dp[m * N + n] = (T)v;
+    __shared__ float red[ACT_ROWS][32][9];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = (blockIdx.x * 32 + c) * 8, left = N - n;
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0.f;
+    if (left > 0)
+        for (int64_t m = (int64_t)blockIdx.y * ACT_ROWS + r; m < M; m += (int64_t)gridDim.y * ACT_ROWS) {
+            float v[8], p[8];
+            load_part<T, 8>(v, dy + m * ldy + n, left);
+            if (auxk != AUX_NONE) {
+                const int64_t at = m * N + n;
+                if (auxk == AUX_U8) {
+                    Pack<uint8_t, 8> q;
+                    load_raw<uint8_t, 8>(q, (const uint8_t*)aux + at, left);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= q.v[e] ? 1.f : slope;
+                } else {
+                    if (auxk == AUX_F16) load_part<f16_t, 8>(p, (const f16_t*)aux + at, left);
+                    else load_part<float, 8>(p, (const float*)aux + at, left);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= dense_act_grad(p[e], act);
                 }
-                s += v;
+                store_part<T, 8>(dp + at, v, left);
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
+        }
     if (part == nullptr) return;
-    red[w][lane] = s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[r][c][e] = s[e];
     __syncthreads();
-    if (w == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    const int col = threadIdx.x, at = blockIdx.x * 256 + col;
+    if (at >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < ACT_ROWS; ++i) t += red[i][col >> 3][col & 7];
+    part[(int64_t)blockIdx.y * N + at] = t;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC, bool DMA>
@@ -475,7 +525,9 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
             granted |= (uint64_t)1 << dev;
         }
     }
-    k<<<dim3((unsigned)ceil_div64(g.N, BN), (unsigned)ceil_div64(g.M, BM), slices), dim3(WM * WN * 64), bytes, s>>>(g);
+    const int64_t tiles = ceil_div64(g.N, BN) * ceil_div64(g.M, BM);
+    if (tiles > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "gemm: %lld tiles", (long long)tiles);
+    k<<<dim3((unsigned)tiles, 1, slices), dim3(WM * WN * 64), bytes, s>>>(g);
     VAE_LAUNCH_CHECK("gemm_k");
     return VAE_OK;
 }
@@ -518,8 +570,13 @@ int gemm(GemmArgs g, float* part, hipStream_t s) {
     }
     int rc;
     if (gemm_small(g.M, g.N)) rc = gemm_inst<T, 64, 64, 2, 2, ARC, BRC, false>(g, slices, s);
-    else if (gemm_large(g.M, g.N) && whole_pieces<T>(g, ARC, BRC)) rc = gemm_inst<T, 256, 256, 2, 2, ARC, BRC, true>(g, slices, s);
-    else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, false>(g, slices, s);
+    else if (whole_pieces<T>(g, ARC, BRC)) {
+        rc = VAE_EINVAL;
+        if constexpr (sizeof(T) == 2) {
+            if (gemm_large(g.M, g.N)) rc = gemm_inst<T, 256, 256, 2, 2, ARC, BRC, true>(g, slices, s);
+            else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, true>(g, slices, s);
+        } else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, true>(g, slices, s);
+    } else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, false>(g, slices, s);
     if (rc != VAE_OK || slices == 1) return rc;
     const int64_t n = (int64_t)g.M * g.N;
     gemm_join_k<T><<<dim3((unsigned)ceil_div64(n, 1024)), dim3(256), 0, s>>>(part, slices, n, (T*)g.c);
@@ -527,9 +584,13 @@ int gemm(GemmArgs g, float* part, hipStream_t s) {
     return VAE_OK;
 }
 
-int dact_rows(int M) {
-    const int64_t n = ceil_div64(M, ACT_ROWS);
-    return (int)(n < 64 ? n : 64);
+// Slices of the rows: about 2048 workgroups in all, 256 at most (rows of partial sums)
+constexpr int DACT_MAX = 256;
+int dact_rows(int64_t M, int64_t N) {
+    int64_t n = ceil_div64(2048, ceil_div64(N, 256));
+    if (n > DACT_MAX) n = DACT_MAX;
+    const int64_t blocks = ceil_div64(M, ACT_ROWS);
+    return (int)(n < blocks ? n : blocks);
 }
 
 struct DenseWs {  // workspace of the backward pass, in floats
@@ -544,7 +605,7 @@ DenseWs dense_ws(int64_t M, int64_t N, int64_t K, int dtype, int act) {
     int ks;
     const int s = gemm_slices(N, K, M, KB / es, &ks);
     w.cols = w.split + (s > 1 ? ceil_div64((int64_t)s * N * K, a) * a : 0);
-    w.total = w.cols + 64 * N;
+    w.total = w.cols + dact_rows(M, N) * N;
     return w;
 }
 
@@ -557,14 +618,14 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
     int64_t lddp = lddy;
     if (auxk != AUX_NONE || db != nullptr) {
         T* out = (T*)(ws + lay.dp);
-        const int ny = dact_rows(M);
+        const int ny = dact_rows(M, N);
         float* cols = db != nullptr ? ws + lay.cols : nullptr;
-        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 64), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, cols, M, N, act, auxk, slope);
+        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, cols, M, N, act, auxk, slope);
         VAE_LAUNCH_CHECK("dense_dact_k");
         if (auxk != AUX_NONE) dp = out, lddp = N;
         if (db != nullptr) {
-            gemm_join_k<T><<<dim3((unsigned)ceil_div64(N, 1024)), dim3(256), 0, s>>>(cols, ny, N, db);
-            VAE_LAUNCH_CHECK("gemm_join_k");
+            part_cols_k<T><<<dim3((unsigned)ceil_div64(N, 64)), dim3(1024), 0, s>>>(cols, ny, N, db, nullptr, N);
+            VAE_LAUNCH_CHECK("part_cols_k");
         }
     }
     if (dx != nullptr) {

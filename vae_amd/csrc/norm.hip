@@ -199,31 +199,6 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_bwd_k(const T* dy, int
     }
 }
 
-// dw, db = column sums of the partial rows, in a fixed order: 64 columns a workgroup, 16 waves that take every 16th row.
-template <typename TW>
-__global__ __launch_bounds__(1024) void norm_part_k(const float* part, int nparts, int C, TW* dw, TW* db) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;  // of 2 C columns: dw, then db
-    float s = 0.f;
-    if (c < 2 * C) {
-#pragma unroll 8
-        for (int r = w; r < nparts; r += 16) s += part[(int64_t)r * 2 * C + c];
-    }
-    red[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && c < 2 * C) {
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s += red[i][lane];
-        if (c < C) {
-            if (dw != nullptr) dw[c] = (TW)s;
-        } else if (db != nullptr) {
-            db[c - C] = (TW)s;
-        }
-    }
-}
-
 // Rows longer than the registers of a workgroup hold: one workgroup a row, the row read once per pass.
 template <typename T, typename TW>
 __global__ __launch_bounds__(1024) void norm_fwd_long_k(const T* x, int64_t ldx, const TW* w, const TW* b, T* y, int64_t ldy,
@@ -344,8 +319,9 @@ int bwd_parts(int64_t rows, int rpb) {
 
 template <typename TW>
 int finish_parts(const NormArgs& a, int nparts) {
-    norm_part_k<TW><<<dim3((unsigned)ceil_div64(2 * (int64_t)a.C, 64)), dim3(1024), 0, a.s>>>(a.part, nparts, a.C, (TW*)a.dw, (TW*)a.db);
-    VAE_LAUNCH_CHECK("norm_part_k");
+    const int64_t n = 2 * (int64_t)a.C;
+    part_cols_k<TW><<<dim3((unsigned)ceil_div64(n, 64)), dim3(1024), 0, a.s>>>(a.part, nparts, n, (TW*)a.dw, (TW*)a.db, a.C);
+    VAE_LAUNCH_CHECK("part_cols_k");
     return VAE_OK;
 }
 

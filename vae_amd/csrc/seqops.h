@@ -71,3 +71,28 @@ __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
     f = r;
     i = e * r;
 }
+
+// Column sums of `rows` rows of n partial sums, in a fixed order: 64 columns a workgroup, 16 waves that take every 16th row.
+// Column c goes to out0[c], or to out1[c - split] from `split` on; a null output is skipped.
+template <typename T>
+__global__ __launch_bounds__(1024) void part_cols_k(const float* part, int rows, int64_t n, T* out0, T* out1, int64_t split) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (c < n) {
+#pragma unroll 8
+        for (int r = w; r < rows; r += 16) s += part[r * n + c];
+    }
+    red[w][lane] = s;
+    __syncthreads();
+    if (w != 0 || c >= n) return;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += red[i][lane];
+    if (c < split) {
+        if (out0 != nullptr) out0[c] = (T)s;
+    } else if (out1 != nullptr) {
+        out1[c - split] = (T)s;
+    }
+}
