@@ -25,35 +25,62 @@ inline int aux_kind(int act, int dtype) {
     return dtype == VAE_T_BF16 ? AUX_F16 : AUX_F32;
 }
 
-__device__ __forceinline__ float dense_act(float p, int act, float slope) {
-    switch (act) {
-        case VAE_ACT_LEAKY: return p > 0.f ? p : p * slope;
-        case VAE_ACT_SIGMOID: {
-            float f, i;
-            gate_pair(p, f, i);
-            return f;
-        }
-        case VAE_ACT_GELU: return 0.5f * p * (1.f + erff(p * 0.70710678f));
-        case VAE_ACT_SILU: {
-            float f, i;
-            gate_pair(p, f, i);
-            return p * f;
-        }
-    }
-    return p;
+// Normal distribution function and exp(-p^2/2): erfc by Abramowitz & Stegun 7.1.26, (a1 t + .. + a5 t^5) exp(-x^2) with
+// t = 1 / (1 + 0.3275911 x), x = |p| / sqrt 2, off by at most 1.5e-7 (the function half of that); no branches.
+__device__ __forceinline__ float normal_cdf(float p, float& e) {
+    const float x = fabsf(p) * 0.70710678f;
+    e = exp_acc(-x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float u = fmaf(t, 1.061405429f, -1.453152027f);
+    u = fmaf(t, u, 1.421413741f);
+    u = fmaf(t, u, -0.284496736f);
+    u = fmaf(t, u, 0.254829592f) * t * 0.5f * e;
+    return p < 0.f ? u : 1.f - u;
 }
-__device__ __forceinline__ float dense_act_grad(float p, int act) {
+
+// act and act' of 8 values: the switch stands outside the loop over them
+__device__ __forceinline__ void dense_act8(float (&v)[8], int act, float slope) {
     float f, i;
     switch (act) {
-        case VAE_ACT_SIGMOID: gate_pair(p, f, i); return f * i;
-        case VAE_ACT_GELU: {
-            if (p > 14.f || p < -14.f) return p > 0.f ? 1.f : 0.f;  // (p exp(-p^2/2) is below fp32's range)
-            return 0.5f * (1.f + erff(p * 0.70710678f)) + p * exp_acc(-0.5f * p * p) * 0.39894228f;
-        }
-        case VAE_ACT_SILU: gate_pair(p, f, i); return f * (1.f + p * i);
+        case VAE_ACT_LEAKY:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] > 0.f ? v[e] : v[e] * slope;
+            break;
+        case VAE_ACT_SIGMOID:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate_pair(v[e], f, i), v[e] = f;
+            break;
+        case VAE_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= normal_cdf(v[e], f);
+            break;
+        case VAE_ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate_pair(v[e], f, i), v[e] *= f;
+            break;
     }
-    return 1.f;
 }
+__device__ __forceinline__ void dense_act_grad8(float (&d)[8], const float (&p)[8], int act) {  // d *= act'(p)
+    float f, i;
+    switch (act) {
+        case VAE_ACT_SIGMOID:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate_pair(p[e], f, i), d[e] *= f * i;
+            break;
+        case VAE_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float c = normal_cdf(p[e], f);
+                d[e] *= fmaf(p[e] * f, 0.39894228f, c);
+            }
+            break;
+        case VAE_ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate_pair(p[e], f, i), d[e] *= f * fmaf(p[e], i, 1.f);
+            break;
+    }
+}
+
 struct GemmArgs {
     const void *a, *b;
     int64_t lda, ldb;
@@ -182,62 +209,72 @@ __device__ __forceinline__ void aux_store8(void* aux, int64_t at, const float (&
     } else if (kind == AUX_F16) {
         float c[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = p[e] > 65504.f ? 65504.f : p[e] < -65504.f ? -65504.f : p[e];
+        for (int e = 0; e < 8; ++e) {
+            c[e] = p[e] > 65504.f ? 65504.f : p[e];  // (a NaN passes)
+            c[e] = c[e] < -65504.f ? -65504.f : c[e];
+        }
         store_part<f16_t, 8>((f16_t*)aux + at, c, left);
     } else if (kind == AUX_F32) {
         store_part<float, 8>((float*)aux + at, p, left);
     }
 }
 
-// bias, what the backward pass needs, activation, residual, and the store of 8 neighbouring columns of a row
-template <typename T>
-__device__ __forceinline__ void finish8(const GemmArgs& g, float (&v)[8], int64_t m, int n) {
-    const int left = g.N - n;
-    if (g.part != nullptr) {
-        store_part<float, 8>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, left);
-        return;
-    }
-    float t[8];
-    if (g.bias != nullptr) {
-        load_part<T, 8>(t, (const T*)g.bias + n, left);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += t[e];
-    }
-    if (g.aux != nullptr) aux_store8(g.aux, m * g.N + n, v, g.auxk, left);
-    if (g.act != VAE_ACT_NONE) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = dense_act(v[e], g.act, g.slope);
-    }
-    if (g.res != nullptr) {
-        load_part<T, 8>(t, (const T*)g.res + m * g.ldr + n, left);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += t[e];
-    }
-    store_part<T, 8>((T*)g.c + m * g.ldc + n, v, left);
-}
-
 // The epilogue of a wave's share of C: acc[i][j][e] is row i * 16 + lane % 16, column j * 16 + lane / 16 * 4 + e.  Two rows of
-// fragments at a time go through LDS (sm: the wave's own part of the tile buffers, free by now), so that lanes hold 8 neighbouring
-// columns and a row leaves in whole lines.
+// fragments at a time go through LDS (sm: the wave's own part of the tile buffers, free by now), so that a lane holds 8 neighbouring
+// columns, the same ones all the time, and a row leaves in whole lines: bias, what the backward pass needs, activation,
+// residual, store.  The residual is loaded two steps ahead.
 template <typename T, int FM, int FN>
 __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)[FM][FN], int m0, int n0, int lane, float* sm) {
-    constexpr int LD = FN * 16 + 4, LPR = FN * 2, RPP = 64 / LPR;  // floats of a row in LDS, lanes a row, rows a pass
+    constexpr int LD = FN * 16 + 4, LPR = FN * 2, RPP = 64 / LPR, PASS = 32 / RPP;  // floats of a row in LDS, lanes a row, rows a pass
+    const int n = n0 + lane % LPR * 8, left = g.N - n, r0 = lane / LPR;
+    const float* mine = sm + r0 * LD + lane % LPR * 8;
+    float bias[8];
+    Pack<T, 8> r1, r2;
 #pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = 0.f, r1.v[e] = r2.v[e] = (T)0.f;
+    const bool plain = g.part != nullptr, has_res = g.res != nullptr && !plain;
+    if (g.bias != nullptr && left > 0 && !plain) load_part<T, 8>(bias, (const T*)g.bias + n, left);
+    const T* res = (const T*)g.res + n;
+    const int end = g.M - m0 < FM * 16 ? g.M - m0 : FM * 16;  // rows of the share that exist
+    if (has_res && left > 0) {
+        if (r0 < end) load_raw<T, 8>(r1, res + (int64_t)(m0 + r0) * g.ldr, left);
+        if (r0 + RPP < end) load_raw<T, 8>(r2, res + (int64_t)(m0 + r0 + RPP) * g.ldr, left);
+    }
+#pragma unroll 1
     for (int i = 0; i < FM; i += 2) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int k = 0; k < FM; k += 2)
+            if (k == i) {  // (the accumulators are registers: each pair of rows has its own code)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(sm + (h * 16 + (lane & 15)) * LD + j * 16 + (lane >> 4) * 4) = acc[i + h][j];
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(sm + (h * 16 + (lane & 15)) * LD + j * 16 + (lane >> 4) * 4) = acc[k + h][j];
+            }
         // (one wave writes and reads: LDS keeps its order)
-        const int n = n0 + lane % LPR * 8;
 #pragma unroll 1
-        for (int r = lane / LPR; r < 32; r += RPP) {
-            const int m = m0 + i * 16 + r;
-            if (m >= g.M || n >= g.N) continue;
-            const float* q = sm + r * LD + lane % LPR * 8;
+        for (int p = 0; p < PASS; ++p) {
+            const int row = i * 16 + p * RPP + r0;
+            const float* q = mine + p * RPP * LD;
             const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+            const Pack<T, 8> r = r1;
+            r1 = r2;
+            if (left <= 0 || row >= end) continue;
+            const int64_t m = m0 + row;
+            if (has_res && row + 2 * RPP < end) load_raw<T, 8>(r2, res + (m + 2 * RPP) * g.ldr, left);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            finish8<T>(g, v, m, n);
+            if (plain) {
+                store_part<float, 8>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, left);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
+            if (g.aux != nullptr) aux_store8(g.aux, m * g.N + n, v, g.auxk, left);
+            dense_act8(v, g.act, g.slope);
+            if (has_res) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += (float)r.v[e];
+            }
+            store_part<T, 8>((T*)g.c + m * g.ldc + n, v, left);
         }
     }
 }
@@ -489,8 +526,7 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
                 } else {
                     if (auxk == AUX_F16) load_part<f16_t, 8>(p, (const f16_t*)aux + at, left);
                     else load_part<float, 8>(p, (const float*)aux + at, left);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= dense_act_grad(p[e], act);
+                    dense_act_grad8(v, p, act);
                 }
                 store_part<T, 8>(dp + at, v, left);
             }

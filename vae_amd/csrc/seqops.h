@@ -67,7 +67,7 @@ __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
     g = g > 87.f ? 87.f : g;
     g = g < -87.f ? -87.f : g;
     const float e = exp_acc(-g);
-    const float r = 1.f / (1.f + e);
+    const float r = __builtin_amdgcn_rcpf(1.f + e);  // (one unit in the last place)
     f = r;
     i = e * r;
 }
