@@ -140,16 +140,28 @@ template <typename T, int R, bool RC, int NT>
 struct Stage {
     static constexpr int V = 16 / sizeof(T), N = R * 8 / NT;
     Pack<T, V> r[N];
+    // A tile inside the operand is loaded without a test an element.  (k contiguous: rows behind the last are read as the last one;
+    // what they give is not stored.)
     __device__ __forceinline__ void load(const T* p, int64_t ld, int r0, int rows, int k0, int kend, int tid) {
+        if (k0 + BK<T>() <= kend && (!RC || r0 + R <= rows)) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int c = tid + j * NT;
+                const int row = r0 + (c >> 3) < rows ? r0 + (c >> 3) : rows - 1;
+                r[j] = *reinterpret_cast<const Pack<T, V>*>(RC ? p + (int64_t)(k0 + c / (R / V)) * ld + r0 + c % (R / V) * V
+                                                               : p + (int64_t)row * ld + k0 + (c & 7) * V);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int c = tid + j * NT;
             if constexpr (!RC) {
                 const int row = r0 + (c >> 3), k = k0 + (c & 7) * V;
-                load_raw<T, V>(r[j], p + (int64_t)row * ld + k, row < rows ? kend - k : 0);
+                load_raw<T, V>(r[j], p + (int64_t)row * ld + k, row < rows ? kend - k : 0, kend >= V);
             } else {
                 const int k = k0 + c / (R / V), row = r0 + c % (R / V) * V;
-                load_raw<T, V>(r[j], p + (int64_t)k * ld + row, k < kend ? rows - row : 0);
+                load_raw<T, V>(r[j], p + (int64_t)k * ld + row, k < kend ? rows - row : 0, rows >= V);
             }
         }
     }
@@ -237,8 +249,8 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
     const T* res = (const T*)g.res + n;
     const int end = g.M - m0 < FM * 16 ? g.M - m0 : FM * 16;  // rows of the share that exist
     if (has_res && left > 0) {
-        if (r0 < end) load_raw<T, 8>(r1, res + (int64_t)(m0 + r0) * g.ldr, left);
-        if (r0 + RPP < end) load_raw<T, 8>(r2, res + (int64_t)(m0 + r0 + RPP) * g.ldr, left);
+        if (r0 < end) load_raw<T, 8>(r1, res + (int64_t)(m0 + r0) * g.ldr, left, g.N >= 8);
+        if (r0 + RPP < end) load_raw<T, 8>(r2, res + (int64_t)(m0 + r0 + RPP) * g.ldr, left, g.N >= 8);
     }
 #pragma unroll 1
     for (int i = 0; i < FM; i += 2) {
@@ -260,7 +272,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
             r1 = r2;
             if (left <= 0 || row >= end) continue;
             const int64_t m = m0 + row;
-            if (has_res && row + 2 * RPP < end) load_raw<T, 8>(r2, res + (m + 2 * RPP) * g.ldr, left);
+            if (has_res && row + 2 * RPP < end) load_raw<T, 8>(r2, res + (m + 2 * RPP) * g.ldr, left, g.N >= 8);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             if (plain) {
                 store_part<float, 8>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, left);
@@ -291,9 +303,11 @@ __device__ __forceinline__ void tile_of(int M, int N, int BM, int BN, int& m, in
     m = grp * 8 + (in - n * h);
 }
 
-// C tile BM x BN by WM x WN waves.  The matrix instruction's first operand is B: a lane then holds four neighbouring columns n of
-// one row m of C.
-template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC>
+// C tile BM x BN by WM x WN waves, for products too small for the kernel below and for operands of any alignment.  The tiles of
+// the operands pass registers, AHEAD of them in flight: with a workgroup or two a CU a tile's loads take longer than its products,
+// and only loads in flight hide that (64 x 4,096 x 4,096 bf16: TIMES).  The matrix instruction's first operand is B: a lane then
+// holds four neighbouring columns n of one row m of C.
+template <typename T, int BM, int BN, int WM, int WN, int AHEAD, bool ARC, bool BRC>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
     constexpr int NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
     extern __shared__ __attribute__((aligned(128))) char lds[];
@@ -303,38 +317,49 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
     m0 *= BM, n0 *= BN;
     const int wm = w % WM * (BM / WM), wn = w / WM * (BN / WN);
     const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
-    Stage<T, BM, ARC, NT> sa;
-    Stage<T, BN, BRC, NT> sb;
+    Stage<T, BM, ARC, NT> sa[AHEAD];
+    Stage<T, BN, BRC, NT> sb[AHEAD];
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sa.load((const T*)g.a, g.lda, m0, g.M, k_lo, k_hi, tid);
-    sb.load((const T*)g.b, g.ldb, n0, g.N, k_lo, k_hi, tid);
-    int cur = 0;
-    for (int k0 = k_lo; k0 < k_hi; k0 += BK<T>(), cur ^= 1) {
-        char *pa = lds + cur * (BM + BN) * KB, *pb = pa + BM * KB;
-        sa.put(pa, tid);
-        sb.put(pb, tid);
-        if (k0 + BK<T>() < k_hi) {
-            sa.load((const T*)g.a, g.lda, m0, g.M, k0 + BK<T>(), k_hi, tid);
-            sb.load((const T*)g.b, g.ldb, n0, g.N, k0 + BK<T>(), k_hi, tid);
-        }
-        lds_barrier();  // (two buffers: the writes of the next tile go to the one that no wave reads any more)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            Pack<T, V> fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = frag<T, BM, ARC>(pa, wm + i * 16, ks, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = frag<T, BN, BRC>(pb, wn + j * 16, ks, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
-        }
+    for (int d = 0; d < AHEAD; ++d) {
+        const int k = k_lo + d * BK<T>();
+        if (k >= k_hi) break;
+        sa[d].load((const T*)g.a, g.lda, m0, g.M, k, k_hi, tid);
+        sb[d].load((const T*)g.b, g.ldb, n0, g.N, k, k_hi, tid);
     }
+    int cur = 0;
+    for (int kk = k_lo; kk < k_hi; kk += AHEAD * BK<T>())
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+            const int k0 = kk + d * BK<T>();
+            if (k0 >= k_hi) break;
+            char *pa = lds + cur * (BM + BN) * KB, *pb = pa + BM * KB;
+            cur ^= 1;
+            sa[d].put(pa, tid);
+            sb[d].put(pb, tid);
+            const int kn = k0 + AHEAD * BK<T>();
+            if (kn < k_hi) {
+                sa[d].load((const T*)g.a, g.lda, m0, g.M, kn, k_hi, tid);
+                sb[d].load((const T*)g.b, g.ldb, n0, g.N, kn, k_hi, tid);
+            }
+            lds_barrier();  // (two buffers: the writes of the next tile go to the one that no wave reads any more)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                Pack<T, V> fa[FM], fb[FN];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) fa[i] = frag<T, BM, ARC>(pa, wm + i * 16, ks, lane);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) fb[j] = frag<T, BN, BRC>(pb, wn + j * 16, ks, lane);
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
+            }
+        }
     __syncthreads();
     store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
@@ -485,6 +510,80 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
     store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
 
+// ---- Few rows (serving) --------------------------------------------------------------------------------------------------
+// y of up to 64 rows: the weight's bytes are the bound, so they are read once and straight into registers.  A workgroup takes 16
+// columns of y (rows of w) and shares k out among its waves; each wave has eight 1-KiB loads in flight, multiplies them on the matrix
+// cores with MF x 16 rows of x (zeros where there are fewer), and the waves' sums meet in LDS.
+constexpr int ROWS_MAX = 64, ROWS_STEPS = 8;
+template <typename T, int MF>
+__global__ __launch_bounds__(MF == 4 ? 512 : 1024) void dense_rows_k(const GemmArgs g, int steps) {  // steps: pieces of 64 bytes of k a wave takes
+    constexpr int V = 16 / sizeof(T), KS = 4 * V;
+    __shared__ float red[MF == 4 ? 8 : 16][MF][16][17];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int n0 = blockIdx.x * 16, r = lane & 15, q = lane >> 4;
+    const int k_lo = w * steps * KS, k_end = g.K - k_lo < steps * KS ? g.K : k_lo + steps * KS;
+    const T* wp = (const T*)g.b + (int64_t)(n0 + r) * g.ldb + q * V;
+    const T* xp = (const T*)g.a + (int64_t)r * g.lda + q * V;
+    const bool live = n0 + r < g.N;
+    f32x4 acc[MF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = k_lo; k0 < k_end; k0 += ROWS_STEPS * KS) {
+        Pack<T, V> fw[ROWS_STEPS], fx[MF][ROWS_STEPS];
+        if (k0 + ROWS_STEPS * KS <= k_end) {
+#pragma unroll
+            for (int t = 0; t < ROWS_STEPS; ++t) load_raw<T, V>(fw[t], wp + k0 + t * KS, live ? V : 0);
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int t = 0; t < ROWS_STEPS; ++t) load_raw<T, V>(fx[i][t], xp + (int64_t)i * 16 * g.lda + k0 + t * KS, i * 16 + r < g.M ? V : 0);
+        } else {
+#pragma unroll
+            for (int t = 0; t < ROWS_STEPS; ++t) load_raw<T, V>(fw[t], wp + k0 + t * KS, live ? k_end - (k0 + t * KS + q * V) : 0, k_end >= V);
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int t = 0; t < ROWS_STEPS; ++t)
+                    load_raw<T, V>(fx[i][t], xp + (int64_t)i * 16 * g.lda + k0 + t * KS, i * 16 + r < g.M ? k_end - (k0 + t * KS + q * V) : 0, k_end >= V);
+        }
+#pragma unroll
+        for (int t = 0; t < ROWS_STEPS; ++t)
+#pragma unroll
+            for (int i = 0; i < MF; ++i) acc[i] = mma16<T>(fw[t], fx[i][t], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[w][i][lane & 15][q * 4 + e] = acc[i][e];
+    __syncthreads();
+    for (int o = threadIdx.x; o < MF * 256; o += blockDim.x) {
+        const int m = o >> 4, n = n0 + (o & 15);
+        if (m >= g.M || n >= g.N) continue;
+        float v[8] = {};
+        for (int k = 0; k < nw; ++k) v[0] += red[k][m >> 4][m & 15][o & 15];
+        if (g.bias != nullptr) v[0] += (float)((const T*)g.bias)[n];
+        if (g.aux != nullptr) aux_store8(g.aux, (int64_t)m * g.N + n, v, g.auxk, 1);
+        dense_act8(v, g.act, g.slope);
+        if (g.res != nullptr) v[0] += (float)((const T*)g.res)[(int64_t)m * g.ldr + n];
+        ((T*)g.c)[(int64_t)m * g.ldc + n] = (T)v[0];
+    }
+}
+
+template <typename T>
+int dense_rows(const GemmArgs& g, hipStream_t s) {
+    constexpr int KS = 64 / sizeof(T);
+    const int pieces = (int)ceil_div64(g.K, KS);
+    int waves = (int)ceil_div64(pieces, ROWS_STEPS);
+    if (waves > (g.M > 32 ? 8 : 16)) waves = g.M > 32 ? 8 : 16;
+    const int steps = (int)ceil_div64(pieces, waves);
+    const dim3 grid((unsigned)ceil_div64(g.N, 16)), block(waves * 64);
+    if (g.M <= 16) dense_rows_k<T, 1><<<grid, block, 0, s>>>(g, steps);
+    else if (g.M <= 32) dense_rows_k<T, 2><<<grid, block, 0, s>>>(g, steps);
+    else dense_rows_k<T, 4><<<grid, block, 0, s>>>(g, steps);
+    VAE_LAUNCH_CHECK("dense_rows_k");
+    return VAE_OK;
+}
+
 // c = sum of the slices of a split product, in a fixed order
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_k(const float* part, int slices, int64_t n, T* c) {
@@ -505,8 +604,8 @@ __global__ __launch_bounds__(256) void gemm_join_k(const float* part, int slices
 // lane, 8 rows at a time, and every gridDim.y-th block of rows; its sums stay in registers until the end.
 constexpr int ACT_ROWS = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, const void* aux, T* dp, float* part, int M, int N, int act, int auxk,
-                                                    float slope) {
+__global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, const void* aux, T* dp, int64_t ldp, float* part, int M, int N, int act,
+                                                    int auxk, float slope) {
     __shared__ float red[ACT_ROWS][32][9];
     const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = (blockIdx.x * 32 + c) * 8, left = N - n;
     float s[8];
@@ -515,20 +614,20 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
     if (left > 0)
         for (int64_t m = (int64_t)blockIdx.y * ACT_ROWS + r; m < M; m += (int64_t)gridDim.y * ACT_ROWS) {
             float v[8], p[8];
-            load_part<T, 8>(v, dy + m * ldy + n, left);
+            load_part<T, 8>(v, dy + m * ldy + n, left, N >= 8);
             if (auxk != AUX_NONE) {
                 const int64_t at = m * N + n;
                 if (auxk == AUX_U8) {
                     Pack<uint8_t, 8> q;
-                    load_raw<uint8_t, 8>(q, (const uint8_t*)aux + at, left);
+                    load_raw<uint8_t, 8>(q, (const uint8_t*)aux + at, left, N >= 8);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] *= q.v[e] ? 1.f : slope;
                 } else {
-                    if (auxk == AUX_F16) load_part<f16_t, 8>(p, (const f16_t*)aux + at, left);
+                    if (auxk == AUX_F16) load_part<f16_t, 8>(p, (const f16_t*)aux + at, left, N >= 8);
                     else load_part<float, 8>(p, (const float*)aux + at, left);
                     dense_act_grad8(v, p, act);
                 }
-                store_part<T, 8>(dp + at, v, left);
+                store_part<T, 8>(dp + m * ldp + n, v, left);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
@@ -551,7 +650,7 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     static_assert(WM * WN * 32 * (BN / WN + 4) * 4 <= bytes, "the epilogue's LDS");
     void (*k)(const GemmArgs);
     if constexpr (DMA) k = gemm_dma_k<T, BM, BN, ARC, BRC>;
-    else k = gemm_k<T, BM, BN, WM, WN, ARC, BRC>;
+    else k = gemm_k<T, BM, BN, WM, WN, BM == 64 ? 4 : 2, ARC, BRC>;
     if (bytes > 65536) {
         static uint64_t granted = 0;  // per device; a race only repeats the call
         int dev = 0;
@@ -629,6 +728,9 @@ int dact_rows(int64_t M, int64_t N) {
     return (int)(n < blocks ? n : blocks);
 }
 
+// dp is ours: its rows start on 16 bytes whatever N is (products of rows that do not take about half as long again)
+int64_t dp_stride(int64_t N, int es) { return ceil_div64(N, 16 / es) * (16 / es); }
+
 struct DenseWs {  // workspace of the backward pass, in floats
     int64_t dp, split, cols, total;
 };
@@ -637,7 +739,7 @@ DenseWs dense_ws(int64_t M, int64_t N, int64_t K, int dtype, int act) {
     const int es = vae_type_size(dtype);
     const int64_t a = 64;
     w.dp = 0;
-    w.split = w.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * N * es, 4), a) * a);
+    w.split = w.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * dp_stride(N, es) * es, 4), a) * a);
     int ks;
     const int s = gemm_slices(N, K, M, KB / es, &ks);
     w.cols = w.split + (s > 1 ? ceil_div64((int64_t)s * N * K, a) * a : 0);
@@ -656,9 +758,9 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
         T* out = (T*)(ws + lay.dp);
         const int ny = dact_rows(M, N);
         float* cols = db != nullptr ? ws + lay.cols : nullptr;
-        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, cols, M, N, act, auxk, slope);
+        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, dp_stride(N, sizeof(T)), cols, M, N, act, auxk, slope);
         VAE_LAUNCH_CHECK("dense_dact_k");
-        if (auxk != AUX_NONE) dp = out, lddp = N;
+        if (auxk != AUX_NONE) dp = out, lddp = dp_stride(N, sizeof(T));
         if (db != nullptr) {
             part_cols_k<T><<<dim3((unsigned)ceil_div64(N, 64)), dim3(1024), 0, s>>>(cols, ny, N, db, nullptr, N);
             VAE_LAUNCH_CHECK("part_cols_k");
@@ -703,6 +805,7 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
     g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
     g.aux = g.auxk == AUX_NONE ? nullptr : aux;
     hipStream_t s = (hipStream_t)stream;
+    if (M <= ROWS_MAX) return dtype == VAE_T_F32 ? dense_rows<float>(g, s) : dtype == VAE_T_BF16 ? dense_rows<bf16_t>(g, s) : dense_rows<f16_t>(g, s);
     if (dtype == VAE_T_F32) return gemm<float, false, false>(g, nullptr, s);
     return dtype == VAE_T_BF16 ? gemm<bf16_t, false, false>(g, nullptr, s) : gemm<f16_t, false, false>(g, nullptr, s);
 }

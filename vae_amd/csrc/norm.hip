@@ -12,80 +12,138 @@
 
 namespace {
 
-constexpr int NORM_MAX_PARTS = 1024;  // workgroups of the backward launch = rows of partials
+// Workgroups of the backward launch = rows of partial sums: their bytes stay small beside the tensors'.
+constexpr int NORM_MAX_PARTS = 1024;
+int64_t norm_parts_cap(int C) {
+    const int64_t n = ((int64_t)1 << 21) / C;
+    return n < 256 ? 256 : n > NORM_MAX_PARTS ? NORM_MAX_PARTS : n;
+}
 
-// sum over the G lanes of a group, valid in each of them
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* sm) {
+// sums over the G lanes of a group, valid in each of them.  sm: a buffer for this sum alone until the workgroup has met at
+// another barrier (one barrier a sum then)
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float* sm) {
     if constexpr (G >= 64) {
-        v = wave_sum(v);
-        if constexpr (G > 64) {
-            const int w = threadIdx.x >> 6;
-            __syncthreads();  // sm may still be read from the sum before
-            if ((threadIdx.x & 63) == 0) sm[w] = v;
-            __syncthreads();
-            v = 0.f;
 #pragma unroll
-            for (int i = 0; i < G / 64; ++i) v += sm[i];
+        for (int n = 0; n < N; ++n) v[n] = wave_sum(v[n]);
+        if constexpr (G > 64) {
+            constexpr int W = G / 64;
+            const int w = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int n = 0; n < N; ++n) sm[w * N + n] = v[n];
+            lds_barrier();
+            const float* mine = sm + w / W * W * N;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                v[n] = 0.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[n] += mine[i * N + n];
+            }
         }
     } else {
 #pragma unroll
-        for (int s = 1; s < G; s <<= 1) v += __shfl_xor(v, s, 64);
+        for (int s = 1; s < G; s <<= 1)
+#pragma unroll
+            for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], s, 64);
     }
-    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_sum1(float v, float* sm) {
+    float t[1] = {v};
+    group_sum<G, 1>(t, sm);
+    return t[0];
 }
 
 template <int G>
 constexpr int norm_threads() { return G > 256 ? G : 256; }
 
+// A lane's NCH pieces of V elements of a row.  The row has more than (NCH - 1) G pieces (the launchers choose so): only the last
+// piece needs a look at where the row ends.  There a lane takes the row's last V elements, whole, and leaves those that its
+// neighbour has too (before `first`) out of the sums; both compute and store the same values for them.  Rows of less than V
+// elements are loaded one by one.
+template <int G, int NCH, int V>
+struct Last {
+    int c, first;  // column of the last piece, first column that counts there
+    __device__ __forceinline__ Last(int lane, int C) {
+        first = ((NCH - 1) * G + lane) * V;
+        c = first + V > C && C >= V ? C - V : first;
+    }
+    __device__ __forceinline__ bool counts(int k, int i, int C) const { return k < NCH - 1 || (c + i >= first && c + i < C); }
+};
+template <typename T, int G, int NCH, int V>
+struct Pieces {
+    Pack<T, V> p[NCH];
+    __device__ __forceinline__ void load(const T* row, int lane, const Last<G, NCH, V>& l, int C) {
+#pragma unroll
+        for (int k = 0; k < NCH - 1; ++k) p[k] = *reinterpret_cast<const Pack<T, V>*>(row + (k * G + lane) * V);
+        if (C >= V) p[NCH - 1] = *reinterpret_cast<const Pack<T, V>*>(row + l.c);
+        else load_raw<T, V>(p[NCH - 1], row + l.c, C - l.c);
+    }
+    __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[k].v[i] = (T)v;
+    }
+};
+template <typename T, int G, int NCH, int V>
+__device__ __forceinline__ void store_pieces(T* row, const float (&v)[NCH][V], int lane, const Last<G, NCH, V>& l, int C) {
+#pragma unroll
+    for (int k = 0; k < NCH - 1; ++k) store_part<T, V>(row + (k * G + lane) * V, v[k], V);
+    if (l.first < C) store_part<T, V>(row + l.c, v[NCH - 1], C - l.c);
+}
+
+// A group goes through every (gridDim.x * groups)-th row; w and b stay in registers (read again a row they would be two thirds of
+// what the loads bring), and the next row is on its way while this one is worked on.
 template <typename T, typename TW, int G, int NCH>
 __global__ __launch_bounds__(norm_threads<G>()) void norm_fwd_k(const T* x, int64_t ldx, const TW* w, const TW* b, T* y, int64_t ldy,
                                                                  float* mean_out, float* rstd_out, int64_t rows, int C, float eps) {
     constexpr int V = 16 / sizeof(T);
-    __shared__ float sm[norm_threads<G>() / 64];
+    __shared__ float sm[2][norm_threads<G>() / 64];
     constexpr int RPB = norm_threads<G>() / G;
-    const int lane = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
-    if (G <= 64 && row >= rows) return;  // (G > 64: one row a workgroup, the grid has exactly `rows`)
-    float v[NCH][V];
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = (k * G + lane) * V;
-        load_part<T, V>(v[k], x + row * ldx + c, C - c);
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += v[k][i];
-    }
+    const int lane = threadIdx.x % G, grp = threadIdx.x / G;
     const float inv = 1.f / (float)C;
-    const float mean = group_sum<G>(s, sm) * inv;
-    float q = 0.f;
+    const Last<G, NCH, V> l(lane, C);
+    Pieces<TW, G, NCH, V> wv, bv;
+    Pieces<T, G, NCH, V> next;
+    int64_t row = (int64_t)blockIdx.x * RPB + grp;
+    next.load(x + (row < rows ? row : rows - 1) * ldx, lane, l, C);
+    if (w != nullptr) wv.load(w, lane, l, C);
+    else wv.fill(1.f);
+    if (b != nullptr) bv.load(b, lane, l, C);
+    else bv.fill(0.f);
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += step, row += step) {  // (all groups of a wave go on together)
+        float v[NCH][V], s = 0.f;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = (k * G + lane) * V;
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float d = v[k][i] - mean;
-            q += c + i < C ? d * d : 0.f;
+            for (int i = 0; i < V; ++i) {
+                v[k][i] = (float)next.p[k].v[i];
+                s += l.counts(k, i, C) ? v[k][i] : 0.f;
+            }
+        if (base + step < rows) next.load(x + (row + step < rows ? row + step : rows - 1) * ldx, lane, l, C);
+        const float mean = group_sum1<G>(s, sm[0]) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[k][i] -= mean;
+                q += l.counts(k, i, C) ? v[k][i] * v[k][i] : 0.f;
+            }
+        const float rstd = 1.f / sqrtf(group_sum1<G>(q, sm[1]) * inv + eps);
+        if (row >= rows) continue;
+        if (lane == 0 && mean_out != nullptr) {
+            mean_out[row] = mean;
+            rstd_out[row] = rstd;
         }
-    }
-    const float rstd = 1.f / sqrtf(group_sum<G>(q, sm) * inv + eps);
-    if (lane == 0 && mean_out != nullptr) {
-        mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = (k * G + lane) * V;
-        if (c >= C) break;
-        float wv[V], bv[V];
-        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c);
-        if (b != nullptr) load_part<TW, V>(bv, b + c, C - c);
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float h = (v[k][i] - mean) * rstd;
-            v[k][i] = (w != nullptr ? h * wv[i] : h) + (b != nullptr ? bv[i] : 0.f);
-        }
-        store_part<T, V>(y + row * ldy + c, v[k], C - c);
+            for (int i = 0; i < V; ++i) v[k][i] = fmaf(v[k][i] * rstd, (float)wv.p[k].v[i], (float)bv.p[k].v[i]);
+        store_pieces<T, G, NCH, V>(y + row * ldy, v, lane, l, C);
     }
 }
 
@@ -96,60 +154,63 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_bwd_k(const T* dy, int
     constexpr int V = 16 / sizeof(T);
     constexpr int NT = norm_threads<G>();
     constexpr int RPB = NT / G;
-    __shared__ float sm[NT / 64];
+    __shared__ float sm[2][2 * NT / 64];
     const int lane = threadIdx.x % G, grp = threadIdx.x / G;
     const float inv = 1.f / (float)C;
-    float wv[NCH][V], dw[NCH][V], db[NCH][V];
+    float dw[NCH][V], db[NCH][V];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-        const int c = (k * G + lane) * V;
-        if (w != nullptr) load_part<TW, V>(wv[k], w + c, C - c);
+    for (int k = 0; k < NCH; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (w == nullptr) wv[k][i] = 1.f;
-            dw[k][i] = db[k][i] = 0.f;
+        for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
+    const Last<G, NCH, V> l(lane, C);
+    Pieces<TW, G, NCH, V> wv;
+    Pieces<T, G, NCH, V> nx, ng;
+    int64_t row = (int64_t)blockIdx.x * RPB + grp;
+    const int64_t r0 = row < rows ? row : rows - 1;
+    nx.load(x + r0 * ldx, lane, l, C);
+    ng.load(dy + r0 * lddy, lane, l, C);
+    float nm = mean_in[r0], nr = rstd_in[r0];
+    if (row >= rows) ng.fill(0.f);
+    if (w != nullptr) wv.load(w, lane, l, C);
+    else wv.fill(1.f);
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int flip = 0;
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += step, row += step, flip ^= 1) {
+        const Pieces<T, G, NCH, V> cx = nx, cg = ng;
+        const float mean = nm, rstd = nr;
+        if (base + step < rows) {
+            const int64_t rn = row + step < rows ? row + step : rows - 1;
+            nx.load(x + rn * ldx, lane, l, C);
+            ng.load(dy + rn * lddy, lane, l, C);
+            nm = mean_in[rn], nr = rstd_in[rn];
+            if (row + step >= rows) ng.fill(0.f);  // (a group without a row: it adds nothing)
         }
-    }
-    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += (int64_t)gridDim.x * RPB) {
-        const int64_t row = base + grp;
-        const bool live = row < rows;  // (groups of one wave may differ here; the shuffles below need all of its lanes)
-        float xv[NCH][V], gv[NCH][V];
+        float s12[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int c = (k * G + lane) * V;
-            load_part<T, V>(xv[k], x + row * ldx + c, live ? C - c : 0);
-            load_part<T, V>(gv[k], dy + row * lddy + c, live ? C - c : 0);
-        }
-        const float mean = live ? mean_in[row] : 0.f, rstd = live ? rstd_in[row] : 0.f;
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int c = (k * G + lane) * V;
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float h = c + i < C ? (xv[k][i] - mean) * rstd : 0.f;
-                xv[k][i] = h;
-                db[k][i] += gv[k][i];
-                dw[k][i] += gv[k][i] * h;
-                gv[k][i] *= wv[k][i];
-                s1 += gv[k][i];
-                s2 += gv[k][i] * h;
+                const float h = ((float)cx.p[k].v[i] - mean) * rstd;
+                const float g = l.counts(k, i, C) ? (float)cg.p[k].v[i] : 0.f;
+                db[k][i] += g;
+                dw[k][i] += g * h;
+                const float gw = g * (float)wv.p[k].v[i];
+                s12[0] += gw;
+                s12[1] += gw * h;
             }
-        }
-        if (dx != nullptr) {
-            s1 = group_sum<G>(s1, sm) * inv;
-            s2 = group_sum<G>(s2, sm) * inv;
-            if (live) {
+        if (dx == nullptr) continue;
+        group_sum<G, 2>(s12, sm[flip]);
+        const float s1 = s12[0] * inv, s2 = s12[1] * inv;
+        if (row >= rows) continue;
+        float o[NCH][V];
 #pragma unroll
-                for (int k = 0; k < NCH; ++k) {
-                    const int c = (k * G + lane) * V;
-                    if (c >= C) break;
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) gv[k][i] = rstd * (gv[k][i] - s1 - xv[k][i] * s2);
-                    store_part<T, V>(dx + row * lddx + c, gv[k], C - c);
-                }
+            for (int i = 0; i < V; ++i) {
+                const float h = ((float)cx.p[k].v[i] - mean) * rstd;
+                o[k][i] = rstd * ((float)cg.p[k].v[i] * (float)wv.p[k].v[i] - s1 - h * s2);
             }
-        }
+        store_pieces<T, G, NCH, V>(dx + row * lddx, o, lane, l, C);
     }
     if (part == nullptr) return;
     // one row of partials a workgroup: [dw | db]
@@ -165,37 +226,37 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_bwd_k(const T* dy, int
                     db[k][i] += __shfl_xor(db[k][i], s, 64);
                 }
     }
-    if constexpr (G <= 64) {
-        constexpr int NW = NT / 64, W = G * NCH * V;  // columns a group holds
+    if constexpr (RPB > 1) {
+        constexpr int U = G < 64 ? 64 : G, NW = NT / U, W = G * NCH * V;  // (the groups of a wave are one by now); columns a group holds
         __shared__ float red[NW - 1][2][W];
-        const int wv_id = threadIdx.x >> 6, l = threadIdx.x & 63;
-        if (wv_id > 0 && l < G) {
+        const int wv_id = threadIdx.x / U, ln = threadIdx.x % U;
+        if (wv_id > 0 && ln < G) {
 #pragma unroll
             for (int k = 0; k < NCH; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    red[wv_id - 1][0][(k * G + l) * V + i] = dw[k][i];
-                    red[wv_id - 1][1][(k * G + l) * V + i] = db[k][i];
+                    red[wv_id - 1][0][(k * G + ln) * V + i] = dw[k][i];
+                    red[wv_id - 1][1][(k * G + ln) * V + i] = db[k][i];
                 }
         }
         __syncthreads();
-        if (wv_id > 0 || l >= G) return;
+        if (wv_id > 0 || ln >= G) return;
 #pragma unroll
         for (int k = 0; k < NCH; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int q = 0; q < NW - 1; ++q) {
-                    dw[k][i] += red[q][0][(k * G + l) * V + i];
-                    db[k][i] += red[q][1][(k * G + l) * V + i];
+                    dw[k][i] += red[q][0][(k * G + ln) * V + i];
+                    db[k][i] += red[q][1][(k * G + ln) * V + i];
                 }
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-        const int c = (k * G + lane) * V;
-        if (c >= C) break;
-        store_part<float, V>(out + c, dw[k], C - c);
-        store_part<float, V>(out + C + c, db[k], C - c);
+        const int c = k < NCH - 1 ? (k * G + lane) * V : l.c;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (l.counts(k, i, C)) out[c + i] = dw[k][i], out[C + c + i] = db[k][i];
     }
 }
 
@@ -204,33 +265,33 @@ template <typename T, typename TW>
 __global__ __launch_bounds__(1024) void norm_fwd_long_k(const T* x, int64_t ldx, const TW* w, const TW* b, T* y, int64_t ldy,
                                                         float* mean_out, float* rstd_out, int C, float eps) {
     constexpr int V = 16 / sizeof(T);
-    __shared__ float sm[16];
+    __shared__ float sm[2][16];
     const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
     float s = 0.f, v[V];
     for (int64_t c = threadIdx.x * V; c < C; c += 1024 * V) {
-        load_part<T, V>(v, xr + c, C - c);
+        load_part<T, V>(v, xr + c, C - c, C >= V);
 #pragma unroll
         for (int i = 0; i < V; ++i) s += v[i];
     }
     const float inv = 1.f / (float)C;
-    const float mean = group_sum<1024>(s, sm) * inv;
+    const float mean = group_sum1<1024>(s, sm[0]) * inv;
     s = 0.f;
     for (int64_t c = threadIdx.x * V; c < C; c += 1024 * V) {
-        load_part<T, V>(v, xr + c, C - c);
+        load_part<T, V>(v, xr + c, C - c, C >= V);
 #pragma unroll
         for (int i = 0; i < V; ++i) s += c + i < C ? (v[i] - mean) * (v[i] - mean) : 0.f;
     }
-    const float rstd = 1.f / sqrtf(group_sum<1024>(s, sm) * inv + eps);
+    const float rstd = 1.f / sqrtf(group_sum1<1024>(s, sm[1]) * inv + eps);
     if (threadIdx.x == 0 && mean_out != nullptr) {
         mean_out[row] = mean;
         rstd_out[row] = rstd;
     }
     for (int64_t c = threadIdx.x * V; c < C; c += 1024 * V) {
         float wv[V], bv[V];
-        load_part<T, V>(v, xr + c, C - c);
-        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c);
-        if (b != nullptr) load_part<TW, V>(bv, b + c, C - c);
+        load_part<T, V>(v, xr + c, C - c, C >= V);
+        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c, C >= V);
+        if (b != nullptr) load_part<TW, V>(bv, b + c, C - c, C >= V);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float h = (v[i] - mean) * rstd;
@@ -244,14 +305,14 @@ template <typename T, typename TW>
 __global__ __launch_bounds__(1024) void norm_bwd_long_k(const T* dy, int64_t lddy, const T* x, int64_t ldx, const TW* w,
                                                         const float* mean_in, const float* rstd_in, T* dx, int64_t lddx, int C) {
     constexpr int V = 16 / sizeof(T);
-    __shared__ float sm[16];
+    __shared__ float sm[2][16];
     const int64_t row = blockIdx.x;
     const float mean = mean_in[row], rstd = rstd_in[row], inv = 1.f / (float)C;
     float s1 = 0.f, s2 = 0.f, xv[V], gv[V], wv[V];
     for (int64_t c = threadIdx.x * V; c < C; c += 1024 * V) {
-        load_part<T, V>(xv, x + row * ldx + c, C - c);
-        load_part<T, V>(gv, dy + row * lddy + c, C - c);
-        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c);
+        load_part<T, V>(xv, x + row * ldx + c, C - c, C >= V);
+        load_part<T, V>(gv, dy + row * lddy + c, C - c, C >= V);
+        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c, C >= V);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float g = w != nullptr ? gv[i] * wv[i] : gv[i];
@@ -259,12 +320,12 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_k(const T* dy, int64_t ldd
             s2 += c + i < C ? g * (xv[i] - mean) * rstd : 0.f;
         }
     }
-    s1 = group_sum<1024>(s1, sm) * inv;
-    s2 = group_sum<1024>(s2, sm) * inv;
+    s1 = group_sum1<1024>(s1, sm[0]) * inv;
+    s2 = group_sum1<1024>(s2, sm[1]) * inv;
     for (int64_t c = threadIdx.x * V; c < C; c += 1024 * V) {
-        load_part<T, V>(xv, x + row * ldx + c, C - c);
-        load_part<T, V>(gv, dy + row * lddy + c, C - c);
-        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c);
+        load_part<T, V>(xv, x + row * ldx + c, C - c, C >= V);
+        load_part<T, V>(gv, dy + row * lddy + c, C - c, C >= V);
+        if (w != nullptr) load_part<TW, V>(wv, w + c, C - c, C >= V);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float g = w != nullptr ? gv[i] * wv[i] : gv[i];
@@ -301,20 +362,15 @@ struct NormArgs {
     hipStream_t s;
 };
 
+// Workgroups of the forward launch: what the chip holds at once (a wave or more a SIMD, eight at most), each with several rows then.
 template <typename T, typename TW, int G, int NCH>
 int fwd_inst(const NormArgs& a) {
     constexpr int NT = norm_threads<G>();
-    norm_fwd_k<T, TW, G, NCH><<<dim3((unsigned)ceil_div64(a.rows, NT / G)), dim3(NT), 0, a.s>>>(
+    const int64_t need = ceil_div64(a.rows, NT / G), most = 256 * (2048 / NT);
+    norm_fwd_k<T, TW, G, NCH><<<dim3((unsigned)(need < most ? need : most)), dim3(NT), 0, a.s>>>(
         (const T*)a.x, a.ldx, (const TW*)a.w, (const TW*)a.b, (T*)a.y, a.ldy, a.mean, a.rstd, a.rows, a.C, a.eps);
     VAE_LAUNCH_CHECK("norm_fwd_k");
     return VAE_OK;
-}
-
-// Workgroups of the backward launch: enough rows a group that the partials stay a few percent of the bytes, at most
-// NORM_MAX_PARTS.
-int bwd_parts(int64_t rows, int rpb) {
-    const int64_t n = ceil_div64(rows, rpb);
-    return (int)(n < NORM_MAX_PARTS ? n : NORM_MAX_PARTS);
 }
 
 template <typename TW>
@@ -329,16 +385,24 @@ template <typename T, typename TW, int G, int NCH>
 int bwd_inst(const NormArgs& a) {
     constexpr int NT = norm_threads<G>();
     const bool cols = a.dw != nullptr || a.db != nullptr;
-    const int n = bwd_parts(a.rows, NT / G);
-    norm_bwd_k<T, TW, G, NCH><<<dim3(n), dim3(NT), 0, a.s>>>((const T*)a.dy, a.lddy, (const T*)a.x, a.ldx, (const TW*)a.w, a.cmean, a.crstd,
+    static int resident = 0;  // workgroups that the chip holds at once (the same on every device; a race only repeats the query)
+    if (resident == 0) {
+        int cu = 0;
+        VAE_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&cu, norm_bwd_k<T, TW, G, NCH>, NT, 0));
+        resident = 256 * (cu < 1 ? 1 : cu);
+    }
+    int64_t n = ceil_div64(a.rows, NT / G);
+    if (n > norm_parts_cap(a.C)) n = norm_parts_cap(a.C);
+    if (n > resident) n = resident;
+    norm_bwd_k<T, TW, G, NCH><<<dim3((unsigned)n), dim3(NT), 0, a.s>>>((const T*)a.dy, a.lddy, (const T*)a.x, a.ldx, (const TW*)a.w, a.cmean, a.crstd,
                                                              (T*)a.dx, a.lddx, cols ? a.part : nullptr, a.rows, a.C);
     VAE_LAUNCH_CHECK("norm_bwd_k");
-    return cols ? finish_parts<TW>(a, n) : VAE_OK;
+    return cols ? finish_parts<TW>(a, (int)n) : VAE_OK;
 }
 
 constexpr int NORM_LONG_SLICES = 64;
 
-// The smallest group that holds the row: G lanes x NCH pieces of 16 bytes.
+// The smallest group that holds the row: G lanes x NCH pieces of 16 bytes, all but the last of them full.
 template <typename T, typename TW>
 int norm_forward_t(const NormArgs& a) {
     constexpr int V = 16 / sizeof(T);
@@ -348,11 +412,12 @@ int norm_forward_t(const NormArgs& a) {
     if (p <= 32) return fwd_inst<T, TW, 32, 1>(a);
     if (p <= 64) return fwd_inst<T, TW, 64, 1>(a);
     if (p <= 128) return fwd_inst<T, TW, 64, 2>(a);
-    if (p <= 256) return fwd_inst<T, TW, 64, 4>(a);
+    if (p <= 256) return fwd_inst<T, TW, 256, 1>(a);
     if (p <= 512) return fwd_inst<T, TW, 256, 2>(a);
-    if (p <= 1024) return fwd_inst<T, TW, 256, 4>(a);
-    if (p <= 2048) return fwd_inst<T, TW, 1024, 2>(a);
-    if (p <= 4096) return fwd_inst<T, TW, 1024, 4>(a);
+    if (p <= 768) return fwd_inst<T, TW, 256, 3>(a);
+    if (p <= 1024) return fwd_inst<T, TW, 512, 2>(a);
+    if (p <= 1536) return fwd_inst<T, TW, 512, 3>(a);
+    if (p <= 2048) return fwd_inst<T, TW, 512, 4>(a);
     norm_fwd_long_k<T, TW><<<dim3((unsigned)a.rows), dim3(1024), 0, a.s>>>((const T*)a.x, a.ldx, (const TW*)a.w, (const TW*)a.b, (T*)a.y,
                                                                            a.ldy, a.mean, a.rstd, a.C, a.eps);
     VAE_LAUNCH_CHECK("norm_fwd_long_k");
@@ -369,9 +434,10 @@ int norm_backward_t(const NormArgs& a) {
     if (p <= 64) return bwd_inst<T, TW, 64, 1>(a);
     if (p <= 128) return bwd_inst<T, TW, 64, 2>(a);
     if (p <= 256) return bwd_inst<T, TW, 256, 1>(a);
-    if (p <= 512) return bwd_inst<T, TW, 256, 2>(a);
+    if (p <= 512) return bwd_inst<T, TW, 512, 1>(a);
     if (p <= 1024) return bwd_inst<T, TW, 1024, 1>(a);
-    if (p <= 2048) return bwd_inst<T, TW, 1024, 2>(a);
+    if (p <= 1536) return bwd_inst<T, TW, 512, 3>(a);
+    if (p <= 2048) return bwd_inst<T, TW, 512, 4>(a);
     if (a.dx != nullptr) {
         norm_bwd_long_k<T, TW><<<dim3((unsigned)a.rows), dim3(1024), 0, a.s>>>((const T*)a.dy, a.lddy, (const T*)a.x, a.ldx, (const TW*)a.w,
                                                                                a.cmean, a.crstd, (T*)a.dx, a.lddx, a.C);
@@ -422,7 +488,7 @@ extern "C" int vae_layer_norm_forward(const void* x, int64_t ldx, const void* w,
 
 extern "C" int64_t vae_layer_norm_workspace_floats(int64_t rows, int C) {
     if (rows < 1 || C < 1) return 0;
-    return 2 * (int64_t)C * (rows < NORM_MAX_PARTS ? rows : NORM_MAX_PARTS);
+    return 2 * (int64_t)C * (rows < norm_parts_cap(C) ? rows : norm_parts_cap(C));
 }
 
 extern "C" int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,

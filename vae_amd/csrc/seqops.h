@@ -16,27 +16,44 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
-// `left` of the N elements at p (the others are 0 and are not read).
+// `left` of the N elements at p (the others are 0 and are not read), as they are in memory.  wide: the row that they end has N
+// elements or more; then its last N are read in one piece and shifted into place (element by element it takes N - 1 loads).
 template <typename T, int N>
-__device__ __forceinline__ void load_part(float (&r)[N], const T* p, int64_t left) {
-    if (left >= N) {
-        const Pack<T, N> q = *reinterpret_cast<const Pack<T, N>*>(p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = (float)q.v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = i < left ? (float)p[i] : 0.f;
-    }
-}
-// ... as they are in memory, for values that are kept a while before they are used
-template <typename T, int N>
-__device__ __forceinline__ void load_raw(Pack<T, N>& r, const T* p, int64_t left) {
+__device__ __forceinline__ void load_raw(Pack<T, N>& r, const T* p, int64_t left, bool wide = false) {
     if (left >= N) {
         r = *reinterpret_cast<const Pack<T, N>*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.v[i] = i < left ? p[i] : (T)0.f;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = (T)0.f;
+    if (left <= 0) return;  // (lanes outside a tensor are common, lanes at its edge are few: only they go on)
+    if constexpr (N * sizeof(T) == 16 || N * sizeof(T) == 8) {
+        if (wide) {
+            r = *reinterpret_cast<const Pack<T, N>*>(p - (N - (int)left));
+            const int sh = (N - (int)left) * (int)sizeof(T) * 8;
+            if constexpr (N * sizeof(T) == 8) {
+                r = __builtin_bit_cast(Pack<T, N>, __builtin_bit_cast(uint64_t, r) >> sh);
+            } else {
+                struct Two { uint64_t lo, hi; };
+                Two t = __builtin_bit_cast(Two, r);
+                t.lo = sh < 64 ? t.lo >> sh | t.hi << (64 - sh) : t.hi >> (sh - 64);
+                t.hi = sh < 64 ? t.hi >> sh : 0;
+                r = __builtin_bit_cast(Pack<T, N>, t);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+        if (i < left) r.v[i] = p[i];
+}
+// ... as fp32
+template <typename T, int N>
+__device__ __forceinline__ void load_part(float (&r)[N], const T* p, int64_t left, bool wide = false) {
+    Pack<T, N> q;
+    load_raw<T, N>(q, p, left, wide);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = (float)q.v[i];
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_part(T* p, const float (&r)[N], int64_t left) {
