@@ -70,7 +70,7 @@ __device__ __forceinline__ void fold_parts(float (&A)[V], float (&H)[V], const G
         load_part<float, V>(ph, a.maps + (2 * (int64_t)p + 1) * n + l.ch, l.left);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            H[v] = pa[v] * H[v] + ph[v];
+            H[v] = fmaf(pa[v], H[v], ph[v]);
             A[v] *= pa[v];
         }
     }
@@ -102,6 +102,31 @@ __device__ __forceinline__ void enter_part(float (&c)[V], const float* first, co
     __syncthreads();
 }
 
+// A wave's S steps of one tensor as they lie in memory.
+template <typename T, int V>
+struct Steps {
+    Pack<T, V> v[GS_S];
+    __device__ __forceinline__ void load(const T* p, int64_t st, int t, int t_end, const GsLane& l, bool full) {
+        const T* q = p + (int64_t)t * st;
+        if (full) {
+#pragma unroll
+            for (int s = 0; s < GS_S; ++s, q += st) v[s] = *reinterpret_cast<const Pack<T, V>*>(q);
+        } else {
+#pragma unroll
+            for (int s = 0; s < GS_S; ++s) load_raw<T, V>(v[s], q + s * st, t + s < t_end ? l.left : 0);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int s = 0; s < GS_S; ++s)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[s].v[i] = (T)0.f;
+    }
+};
+// Do all lanes of the wave have all their features and the steps t .. t + S - 1 in their sequences?
+template <int V>
+__device__ __forceinline__ bool gs_full(const GsLane& l, int t) { return __all(l.left >= V && t + GS_S <= l.len); }
+
 // SUM: leave the part's map only.
 template <typename T, int V, int W, bool SUM>
 __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
@@ -114,6 +139,10 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
     const int t_lo = (int)blockIdx.y * a.part_steps;
     const int t_hi = a.T - t_lo < a.part_steps ? a.T : t_lo + a.part_steps;
     float c[V], pA[V];
+    Steps<T, V> xr, gr;
+    bool full = gs_full<V>(l, t_lo + w * GS_S);
+    xr.load(x, a.xt, t_lo + w * GS_S, l.len, l, full);
+    gr.load(g, a.gt, t_lo + w * GS_S, l.len, l, full);
     if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = 0.f, pA[v] = 1.f;
@@ -122,16 +151,7 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
     }
     int flip = 0;
     for (int t0 = t_lo; t0 < t_hi; t0 += W * GS_S, flip ^= 1) {
-        if (!SUM && a.kept != nullptr && w == 0 && l.left > 0) store_part<float, V>(a.kept + (int64_t)(t0 / GS_TILE) * a.B * a.D + l.ch, c, l.left);
         const int tw = t0 + w * GS_S;
-        Pack<T, V> xr[GS_S], gr[GS_S];
-#pragma unroll
-        for (int s = 0; s < GS_S; ++s) {
-            const int64_t t = tw + s;
-            const int left = t < l.len ? l.left : 0;
-            load_raw<T, V>(xr[s], x + t * a.xt, left);
-            load_raw<T, V>(gr[s], g + t * a.gt, left);
-        }
         float f[GS_S][V], b[GS_S][V], A[V], H[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f;
@@ -140,11 +160,28 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float i;
-                gate_pair((float)gr[s].v[v], f[s][v], i);
-                b[s][v] = i * (float)xr[s].v[v];
-                if (tw + s >= l.len) f[s][v] = 1.f, b[s][v] = 0.f;
+                gate_pair((float)gr.v[s].v[v], f[s][v], i);
+                b[s][v] = i * (float)xr.v[s].v[v];
+            }
+        if (!full) {  // steps behind the end hold the state
+#pragma unroll
+            for (int s = 0; s < GS_S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (tw + s >= l.len) f[s][v] = 1.f, b[s][v] = 0.f;
+        }
+        const bool stores_full = full;
+        if (t0 + W * GS_S < t_hi) {  // the next tile's loads run while this one is worked on
+            full = gs_full<V>(l, tw + W * GS_S);
+            xr.load(x, a.xt, tw + W * GS_S, l.len, l, full);
+            gr.load(g, a.gt, tw + W * GS_S, l.len, l, full);
+        }
+#pragma unroll
+        for (int s = 0; s < GS_S; ++s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
                 A[v] *= f[s][v];
-                H[v] = f[s][v] * H[v] + b[s][v];
+                H[v] = fmaf(f[s][v], H[v], b[s][v]);
             }
         if constexpr (W > 1) {
             float* m = lds[flip];
@@ -153,7 +190,7 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
                 m[(w * 2 + 0) * 64 * V + v * 64 + lane] = A[v];
                 m[(w * 2 + 1) * 64 * V + v * 64 + lane] = H[v];
             }
-            __syncthreads();
+            lds_barrier();
         }
         // the state before this wave's steps, and the one behind the tile
         float h[V];
@@ -164,20 +201,28 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
                 if (k == w) h[v] = c[v];
                 const float ka = W > 1 ? lds[flip][(k * 2 + 0) * 64 * V + v * 64 + lane] : A[v];
                 const float kh = W > 1 ? lds[flip][(k * 2 + 1) * 64 * V + v * 64 + lane] : H[v];
-                c[v] = ka * c[v] + kh;
+                c[v] = fmaf(ka, c[v], kh);
                 if constexpr (SUM) pA[v] *= ka;
             }
         if constexpr (!SUM) {
+            if (a.kept != nullptr && tw % GS_TILE == 0 && tw < a.T && l.left > 0)
+                store_part<float, V>(a.kept + (int64_t)(tw / GS_TILE) * a.B * a.D + l.ch, h, l.left);
+            T* yp = y + (int64_t)tw * a.D;
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s) {
-                const int64_t t = tw + s;
+            for (int s = 0; s < GS_S; ++s, yp += a.D) {
                 float o[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    h[v] = f[s][v] * h[v] + b[s][v];
-                    o[v] = t < l.len ? h[v] : 0.f;
+                    h[v] = fmaf(f[s][v], h[v], b[s][v]);
+                    o[v] = h[v];
                 }
-                if (t < a.T && l.left > 0) store_part<T, V>(y + t * a.D, o, l.left);
+                if (stores_full) {
+                    store_part<T, V>(yp, o, V);
+                } else if (tw + s < a.T && l.left > 0) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] = tw + s < l.len ? o[v] : 0.f;
+                    store_part<T, V>(yp, o, l.left);
+                }
             }
         }
     }
@@ -204,7 +249,24 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
     T* dg = (T*)a.dg + (int64_t)l.b * a.T * a.D + l.d;
     const int t_lo = (int)blockIdx.y * a.part_steps;
     const int t_hi = a.T - t_lo < a.part_steps ? a.T : t_lo + a.part_steps;
-    float c[V], pA[V];  // c: f_{t+1} dh_{t+1} behind the tile (dh_last behind the series)
+    const int last = t_lo + (t_hi - 1 - t_lo) / (W * GS_S) * (W * GS_S);
+    float c[V], pA[V], hn[V];  // c: f_{t+1} dh_{t+1} behind the tile (dh_last behind the series); hn: state before the next tile
+    Steps<T, V> xr, gr, dr;
+    xr.zero(), dr.zero();
+    bool full = gs_full<V>(l, last + w * GS_S);
+    auto fetch = [&](int t0) {
+        const int tw = t0 + w * GS_S;
+        gr.load(g, a.gt, tw, l.len, l, full);
+        if (a.dy != nullptr) dr.load(dy, a.dyt, tw, l.len, l, full);
+        if constexpr (!SUM) {
+            xr.load(x, a.xt, tw, l.len, l, full);
+            const float* from = t0 == 0 ? a.h0 : a.kept + (int64_t)(t0 / GS_TILE) * a.B * a.D;
+#pragma unroll
+            for (int v = 0; v < V; ++v) hn[v] = 0.f;
+            if (from != nullptr) ld_state<V>(hn, from, l);
+        }
+    };
+    fetch(last);
     if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = 0.f, pA[v] = 1.f;
@@ -212,43 +274,42 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
         enter_part<V, W, true>(c, a.dhl, a, l, lds[0]);
     }
     int flip = 0;
-    const int last = t_lo + (t_hi - 1 - t_lo) / (W * GS_S) * (W * GS_S);
     for (int t0 = last; t0 >= t_lo; t0 -= W * GS_S, flip ^= 1) {
         const int tw = t0 + w * GS_S;
-        float hs[V];  // state before the tile
-        if constexpr (!SUM) {
-            const float* from = t0 == 0 ? a.h0 : a.kept + (int64_t)(t0 / GS_TILE) * a.B * a.D;
+        float f[GS_S][V], i[GS_S][V], xs[GS_S][V], ds[GS_S][V], hs[V], A[V], H[V], Q[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) hs[v] = 0.f;
-            if (from != nullptr) ld_state<V>(hs, from, l);
-        }
-        Pack<T, V> xr[GS_S], gr[GS_S], dr[GS_S];
-#pragma unroll
-        for (int s = 0; s < GS_S; ++s) {
-            const int64_t t = tw + s;
-            const int left = t < l.len ? l.left : 0;
-            if constexpr (!SUM) load_raw<T, V>(xr[s], x + t * a.xt, left);
-            load_raw<T, V>(gr[s], g + t * a.gt, left);
-            load_raw<T, V>(dr[s], dy + t * a.dyt, a.dy != nullptr ? left : 0);
-        }
-        float f[GS_S][V], i[GS_S][V], A[V], H[V], Q[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f;
+        for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f, Q[v] = 0.f, hs[v] = SUM ? 0.f : hn[v];
 #pragma unroll
         for (int s = 0; s < GS_S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gate_pair((float)gr[s].v[v], f[s][v], i[s][v]);
-                if (tw + s >= l.len) f[s][v] = 1.f, i[s][v] = 0.f;
-                A[v] *= f[s][v];
-                if constexpr (!SUM) H[v] = f[s][v] * H[v] + i[s][v] * (float)xr[s].v[v];
+                gate_pair((float)gr.v[s].v[v], f[s][v], i[s][v]);
+                if constexpr (!SUM) xs[s][v] = (float)xr.v[s].v[v];
+                ds[s][v] = (float)dr.v[s].v[v];
             }
+        if (!full) {  // (what is not read is 0)
 #pragma unroll
-        for (int v = 0; v < V; ++v) Q[v] = 0.f;
+            for (int s = 0; s < GS_S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (tw + s >= l.len) f[s][v] = 1.f, i[s][v] = 0.f;
+        }
+        const bool stores_full = full;
+        if (t0 - W * GS_S >= t_lo) {
+            full = gs_full<V>(l, tw - W * GS_S);
+            fetch(t0 - W * GS_S);
+        }
+#pragma unroll
+        for (int s = 0; s < GS_S; ++s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                A[v] *= f[s][v];
+                if constexpr (!SUM) H[v] = fmaf(f[s][v], H[v], i[s][v] * xs[s][v]);
+            }
 #pragma unroll
         for (int s = GS_S - 1; s >= 0; --s)
 #pragma unroll
-            for (int v = 0; v < V; ++v) Q[v] = f[s][v] * (Q[v] + (float)dr[s].v[v]);
+            for (int v = 0; v < V; ++v) Q[v] = f[s][v] * (Q[v] + ds[s][v]);
         if constexpr (W > 1) {
             float* m = lds[flip];
 #pragma unroll
@@ -257,7 +318,7 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                 m[(w * M + 1) * 64 * V + v * 64 + lane] = Q[v];
                 if constexpr (!SUM) m[(w * M + 2) * 64 * V + v * 64 + lane] = H[v];
             }
-            __syncthreads();
+            lds_barrier();
         }
         float q[V];
 #pragma unroll
@@ -267,7 +328,7 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                 if (k == w) q[v] = c[v];
                 const float ka = W > 1 ? lds[flip][(k * M + 0) * 64 * V + v * 64 + lane] : A[v];
                 const float kq = W > 1 ? lds[flip][(k * M + 1) * 64 * V + v * 64 + lane] : Q[v];
-                c[v] = ka * c[v] + kq;
+                c[v] = fmaf(ka, c[v], kq);
                 if constexpr (SUM) pA[v] *= ka;
             }
         if constexpr (!SUM) {
@@ -276,30 +337,37 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                 for (int k = 0; k < W - 1; ++k)
 #pragma unroll
                     for (int v = 0; v < V; ++v)
-                        if (k < w) hs[v] = lds[flip][(k * M + 0) * 64 * V + v * 64 + lane] * hs[v] + lds[flip][(k * M + 2) * 64 * V + v * 64 + lane];
+                        if (k < w) hs[v] = fmaf(lds[flip][(k * M + 0) * 64 * V + v * 64 + lane], hs[v], lds[flip][(k * M + 2) * 64 * V + v * 64 + lane]);
             }
-            float hp[GS_S][V];
+            // forward through the wave's steps: xs becomes h_{t-1} - x_t
 #pragma unroll
             for (int s = 0; s < GS_S; ++s)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    hp[s][v] = hs[v];
-                    hs[v] = f[s][v] * hs[v] + i[s][v] * (float)xr[s].v[v];
+                    const float h = fmaf(f[s][v], hs[v], i[s][v] * xs[s][v]);
+                    xs[s][v] = hs[v] - xs[s][v];
+                    hs[v] = h;
                 }
+            T *xp = dx + (int64_t)(tw + GS_S - 1) * a.D, *gp = dg + (int64_t)(tw + GS_S - 1) * a.D;
 #pragma unroll
-            for (int s = GS_S - 1; s >= 0; --s) {
-                const int64_t t = tw + s;
+            for (int s = GS_S - 1; s >= 0; --s, xp -= a.D, gp -= a.D) {
                 float ox[V], og[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float dh = q[v] + (float)dr[s].v[v];
+                    const float dh = q[v] + ds[s][v];
                     q[v] = f[s][v] * dh;
-                    ox[v] = t < l.len ? i[s][v] * dh : 0.f;
-                    og[v] = t < l.len ? dh * (hp[s][v] - (float)xr[s].v[v]) * f[s][v] * i[s][v] : 0.f;
+                    ox[v] = i[s][v] * dh;
+                    og[v] = q[v] * xs[s][v] * i[s][v];
                 }
-                if (t < a.T && l.left > 0) {
-                    if (a.dx != nullptr) store_part<T, V>(dx + t * a.D, ox, l.left);
-                    if (a.dg != nullptr) store_part<T, V>(dg + t * a.D, og, l.left);
+                if (stores_full) {
+                    if (a.dx != nullptr) store_part<T, V>(xp, ox, V);
+                    if (a.dg != nullptr) store_part<T, V>(gp, og, V);
+                } else if (tw + s < a.T && l.left > 0) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        if (tw + s >= l.len) ox[v] = og[v] = 0.f;
+                    if (a.dx != nullptr) store_part<T, V>(xp, ox, l.left);
+                    if (a.dg != nullptr) store_part<T, V>(gp, og, l.left);
                 }
             }
         }
@@ -316,41 +384,62 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
 
 int64_t gs_columns(int B, int D, int V) { return ceil_div64((int64_t)B * ((D + V - 1) / V), 64); }
 
-// Parts of the time axis: one where the channels alone give enough workgroups.
-constexpr int GS_V16 = 4, GS_V32 = 2;  // features a lane holds: 8 bytes
-int gs_parts(int B, int T, int D, int esize, int* part_steps) {
-    const int64_t cols = gs_columns(B, D, esize == 2 ? GS_V16 : GS_V32);
-    const int64_t tiles = ceil_div64(T, GS_TILE);
-    int64_t p = cols >= 512 ? 1 : ceil_div64(1024, cols);
-    if (p > GS_MAX_PARTS) p = GS_MAX_PARTS;
-    if (p > tiles) p = tiles;
-    const int64_t per = ceil_div64(tiles, p);
-    *part_steps = (int)(per * GS_TILE);
-    return (int)ceil_div64(tiles, per);
+// What a launch looks like: V features a lane (8 bytes where there are channels enough, fewer until there are 256 columns of
+// workgroups), W waves a workgroup, parts of the time axis.
+struct GsPlan {
+    int V, W, parts, part_steps;
+};
+GsPlan gs_plan(int B, int T, int D, int esize) {
+    GsPlan p;
+    p.V = esize == 2 ? 4 : 2;
+    while (p.V > 1 && gs_columns(B, D, p.V) < 256) p.V >>= 1;
+    const int64_t cols = gs_columns(B, D, p.V);
+    p.W = T <= GS_S ? 1 : T <= 4 * GS_S ? 4 : cols >= 512 || T <= GS_TILE || p.V > 1 ? 8 : 16;
+    const int64_t tile = p.W * GS_S, tiles = ceil_div64(T, tile);
+    int64_t n = cols >= 192 ? 1 : ceil_div64(512, cols);
+    if (n > GS_MAX_PARTS) n = GS_MAX_PARTS;
+    if (n > tiles) n = tiles;
+    const int64_t per = ceil_div64(tiles, n);
+    p.part_steps = (int)(per * tile);
+    p.parts = (int)ceil_div64(tiles, per);
+    return p;
 }
 
-template <typename T, int V, bool FWD>
+template <typename T, int V, int W, bool FWD>
 int gs_launch(const GsArgs& a) {
     const dim3 grid((unsigned)gs_columns(a.B, a.D, V), a.parts);
-#define VAE_GS(W)                                                                  \
-    do {                                                                           \
-        if (FWD) gscan_fwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);   \
-        else gscan_bwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);       \
-    } while (0)
-    if (a.T <= GS_S) VAE_GS(1);
-    else if (a.T <= 2 * GS_S) VAE_GS(2);
-    else if (a.T <= 4 * GS_S) VAE_GS(4);
-    else {
+    if constexpr (W >= 8) {
         if (a.parts > 1) {
-            if (FWD) gscan_fwd_k<T, V, 8, true><<<grid, dim3(512), 0, a.s>>>(a);
-            else gscan_bwd_k<T, V, 8, true><<<grid, dim3(512), 0, a.s>>>(a);
+            if (FWD) gscan_fwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
+            else gscan_bwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
             VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k (maps)" : "gscan_bwd_k (maps)");
         }
-        VAE_GS(8);
     }
-#undef VAE_GS
+    if (FWD) gscan_fwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
+    else gscan_bwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
     VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k" : "gscan_bwd_k");
     return VAE_OK;
+}
+
+template <typename T, bool FWD>
+int gs_run(GsArgs& a) {
+    const GsPlan p = gs_plan(a.B, a.T, a.D, sizeof(T));
+    a.parts = p.parts, a.part_steps = p.part_steps;
+    if (a.parts > 1 && a.maps == nullptr) VAE_FAIL(VAE_EINVAL, "gated_scan: null workspace");
+#define VAE_GS(NV)                                                      \
+    if (p.V == NV) {                                                    \
+        if (p.W == 1) return gs_launch<T, NV, 1, FWD>(a);               \
+        if (p.W == 4) return gs_launch<T, NV, 4, FWD>(a);               \
+        if (p.W == 8) return gs_launch<T, NV, 8, FWD>(a);               \
+        if constexpr (NV == 1) return gs_launch<T, 1, 16, FWD>(a);      \
+    }
+    VAE_GS(1)
+    VAE_GS(2)
+    if constexpr (sizeof(T) == 2) {
+        VAE_GS(4)
+    }
+#undef VAE_GS
+    VAE_FAIL(VAE_EINVAL, "gated_scan: no launch for V = %d, W = %d", p.V, p.W);
 }
 
 int gs_check(const char* what, int B, int T, int D, int dtype) {
@@ -369,8 +458,7 @@ extern "C" int64_t vae_gated_scan_kept_floats(int B, int T, int D) {
 
 extern "C" int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype) {
     if (B < 1 || T < 1 || D < 1 || vae_type_size(dtype) == 0) return 0;
-    int steps;
-    const int p = gs_parts(B, T, D, vae_type_size(dtype), &steps);
+    const int p = gs_plan(B, T, D, vae_type_size(dtype)).parts;
     return p > 1 ? 2 * (int64_t)p * B * D : 0;
 }
 
@@ -380,12 +468,11 @@ extern "C" int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st,
     if (int rc = gs_check("gated_scan_forward", B, T, D, dtype)) return rc;
     if (B == 0) return VAE_OK;
     GsArgs a = {};
-    a.parts = gs_parts(B, T, D, vae_type_size(dtype), &a.part_steps);
-    if (x == nullptr || gate == nullptr || y == nullptr || (a.parts > 1 && workspace == nullptr)) VAE_FAIL(VAE_EINVAL, "gated_scan_forward: null buffer");
+    if (x == nullptr || gate == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "gated_scan_forward: null buffer");
     a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st, a.h0 = h0, a.lengths = lengths, a.y = y, a.hl = h_last;
     a.kept = T > GS_TILE ? kept : nullptr, a.maps = workspace, a.B = B, a.T = T, a.D = D, a.s = (hipStream_t)stream;
-    if (dtype == VAE_T_F32) return gs_launch<float, GS_V32, true>(a);
-    return dtype == VAE_T_BF16 ? gs_launch<bf16_t, GS_V16, true>(a) : gs_launch<f16_t, GS_V16, true>(a);
+    if (dtype == VAE_T_F32) return gs_run<float, true>(a);
+    return dtype == VAE_T_BF16 ? gs_run<bf16_t, true>(a) : gs_run<f16_t, true>(a);
 }
 
 extern "C" int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last, const void* x, int64_t x_sb,
@@ -395,12 +482,11 @@ extern "C" int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy
     if (int rc = gs_check("gated_scan_backward", B, T, D, dtype)) return rc;
     if (B == 0) return VAE_OK;
     GsArgs a = {};
-    a.parts = gs_parts(B, T, D, vae_type_size(dtype), &a.part_steps);
-    if (x == nullptr || gate == nullptr || (T > GS_TILE && kept == nullptr) || (a.parts > 1 && workspace == nullptr))
+    if (x == nullptr || gate == nullptr || (T > GS_TILE && kept == nullptr))
         VAE_FAIL(VAE_EINVAL, "gated_scan_backward: null buffer");
     a.dy = dy, a.dyb = dy_sb, a.dyt = dy_st, a.dhl = dh_last, a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st;
     a.h0 = h0, a.lengths = lengths, a.kept = const_cast<float*>(kept), a.dx = dx, a.dg = dgate, a.dh0 = dh0, a.maps = workspace;
     a.B = B, a.T = T, a.D = D, a.s = (hipStream_t)stream;
-    if (dtype == VAE_T_F32) return gs_launch<float, GS_V32, false>(a);
-    return dtype == VAE_T_BF16 ? gs_launch<bf16_t, GS_V16, false>(a) : gs_launch<f16_t, GS_V16, false>(a);
+    if (dtype == VAE_T_F32) return gs_run<float, false>(a);
+    return dtype == VAE_T_BF16 ? gs_run<bf16_t, false>(a) : gs_run<f16_t, false>(a);
 }
