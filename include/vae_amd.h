@@ -355,8 +355,8 @@ int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
 
 /* Gated linear recurrence over B sequences of T steps of D features: f = sigmoid(gate), h_t = f h_{t-1} + (1 - f) x_t, y_t = h_t.
  * x, gate, dy: element (b, t, d) at b*sb + t*st + d; y, dx, dgate: dense B x T x D.  h0, h_last, dh_last, dh0: B x D floats,
- * optional (absent: zeros).  lengths (B, optional, clamped to 0..T): steps at and behind a sequence's length hold the state; x, gate
- * and dy are not read there, y, dx and dgate are 0; h_last is the state behind the last step that counts.
+ * optional (absent: zeros).  lengths (B, optional, clamped to 0..T): steps at and behind a sequence's length hold the state, whatever
+ * x, gate and dy contain there; y, dx and dgate are 0 there; h_last is the state behind the last step that counts.
  * kept (vae_gated_scan_kept_floats; NULL when no backward pass follows): states that the backward pass starts its tiles from. */
 int64_t vae_gated_scan_kept_floats(int B, int T, int D);
 int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype);

@@ -36,27 +36,38 @@ struct GsArgs {
     hipStream_t s;
 };
 
+// A lane's V features of one sequence.  V divides nothing here: the last lane of a sequence takes its last V features, whole (V <= D),
+// and shares some with its neighbour; both compute and store the same values for them.  Lanes behind the last channel work on the
+// last one too and store nothing.
 struct GsLane {
-    int b, d, left, len;
+    int b, d, len, t_max;  // t_max: the last step that may be read
+    bool stores;
     int64_t ch;
 };
 template <int V>
 __device__ __forceinline__ GsLane gs_lane(const GsArgs& a) {
     const int dv = (a.D + V - 1) / V;
-    const int64_t q = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    int64_t q = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     GsLane l;
+    l.stores = q < (int64_t)a.B * dv;
+    if (!l.stores) q = (int64_t)a.B * dv - 1;
     l.b = (int)(q / dv);
     l.d = (int)(q - (int64_t)l.b * dv) * V;
-    l.left = l.b < a.B ? a.D - l.d : 0;
-    l.len = l.left > 0 ? (a.lengths != nullptr ? a.lengths[l.b] : a.T) : 0;
-    if (l.len > a.T) l.len = a.T;
+    if (l.d > a.D - V) l.d = a.D - V;
+    l.len = a.lengths != nullptr ? a.lengths[l.b] : a.T;
+    l.len = l.len > a.T ? a.T : l.len < 0 ? 0 : l.len;
+    l.t_max = l.len > 0 ? l.len - 1 : 0;
     l.ch = (int64_t)l.b * a.D + l.d;
     return l;
 }
 
 template <int V>
 __device__ __forceinline__ void ld_state(float (&r)[V], const float* p, const GsLane& l) {
-    load_part<float, V>(r, p + l.ch, l.left);
+    load_part<float, V>(r, p + l.ch, V);
+}
+template <int V>
+__device__ __forceinline__ void st_state(float* p, const float (&r)[V], const GsLane& l) {
+    store_part<float, V>(p + l.ch, r, V);
 }
 
 // (A, H) of the maps of parts [lo, hi) of this lane's channels, in time order (REV: from the last to the first)
@@ -66,8 +77,8 @@ __device__ __forceinline__ void fold_parts(float (&A)[V], float (&H)[V], const G
     for (int k = lo; k < hi; ++k) {
         const int p = REV ? a.parts - 1 - k : k;
         float pa[V], ph[V];
-        load_part<float, V>(pa, a.maps + (2 * (int64_t)p) * n + l.ch, l.left);
-        load_part<float, V>(ph, a.maps + (2 * (int64_t)p + 1) * n + l.ch, l.left);
+        ld_state<V>(pa, a.maps + (2 * (int64_t)p) * n, l);
+        ld_state<V>(ph, a.maps + (2 * (int64_t)p + 1) * n, l);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             H[v] = fmaf(pa[v], H[v], ph[v]);
@@ -102,18 +113,18 @@ __device__ __forceinline__ void enter_part(float (&c)[V], const float* first, co
     __syncthreads();
 }
 
-// A wave's S steps of one tensor as they lie in memory.
+// A wave's S steps of one tensor as they lie in memory; steps behind the sequence's end are read as its last one and not used.
 template <typename T, int V>
 struct Steps {
     Pack<T, V> v[GS_S];
-    __device__ __forceinline__ void load(const T* p, int64_t st, int t, int t_end, const GsLane& l, bool full) {
-        const T* q = p + (int64_t)t * st;
+    __device__ __forceinline__ void load(const T* p, int64_t st, int t, const GsLane& l, bool full) {
         if (full) {
+            const T* q = p + (int64_t)t * st;
 #pragma unroll
             for (int s = 0; s < GS_S; ++s, q += st) v[s] = *reinterpret_cast<const Pack<T, V>*>(q);
         } else {
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s) load_raw<T, V>(v[s], q + s * st, t + s < t_end ? l.left : 0);
+            for (int s = 0; s < GS_S; ++s) v[s] = *reinterpret_cast<const Pack<T, V>*>(p + (int64_t)(t + s < l.t_max ? t + s : l.t_max) * st);
         }
     }
     __device__ __forceinline__ void zero() {
@@ -123,9 +134,8 @@ struct Steps {
             for (int i = 0; i < V; ++i) v[s].v[i] = (T)0.f;
     }
 };
-// Do all lanes of the wave have all their features and the steps t .. t + S - 1 in their sequences?
-template <int V>
-__device__ __forceinline__ bool gs_full(const GsLane& l, int t) { return __all(l.left >= V && t + GS_S <= l.len); }
+// Do all lanes of the wave have the steps t .. t + S - 1 in their sequences, and store what they compute?
+__device__ __forceinline__ bool gs_full(const GsLane& l, int t) { return __all(l.stores && t + GS_S <= l.len); }
 
 // SUM: leave the part's map only.
 template <typename T, int V, int W, bool SUM>
@@ -140,9 +150,9 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
     const int t_hi = a.T - t_lo < a.part_steps ? a.T : t_lo + a.part_steps;
     float c[V], pA[V];
     Steps<T, V> xr, gr;
-    bool full = gs_full<V>(l, t_lo + w * GS_S);
-    xr.load(x, a.xt, t_lo + w * GS_S, l.len, l, full);
-    gr.load(g, a.gt, t_lo + w * GS_S, l.len, l, full);
+    bool full = gs_full(l, t_lo + w * GS_S);
+    xr.load(x, a.xt, t_lo + w * GS_S, l, full);
+    gr.load(g, a.gt, t_lo + w * GS_S, l, full);
     if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = 0.f, pA[v] = 1.f;
@@ -172,9 +182,9 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
         }
         const bool stores_full = full;
         if (t0 + W * GS_S < t_hi) {  // the next tile's loads run while this one is worked on
-            full = gs_full<V>(l, tw + W * GS_S);
-            xr.load(x, a.xt, tw + W * GS_S, l.len, l, full);
-            gr.load(g, a.gt, tw + W * GS_S, l.len, l, full);
+            full = gs_full(l, tw + W * GS_S);
+            xr.load(x, a.xt, tw + W * GS_S, l, full);
+            gr.load(g, a.gt, tw + W * GS_S, l, full);
         }
 #pragma unroll
         for (int s = 0; s < GS_S; ++s)
@@ -205,8 +215,7 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
                 if constexpr (SUM) pA[v] *= ka;
             }
         if constexpr (!SUM) {
-            if (a.kept != nullptr && tw % GS_TILE == 0 && tw < a.T && l.left > 0)
-                store_part<float, V>(a.kept + (int64_t)(tw / GS_TILE) * a.B * a.D + l.ch, h, l.left);
+            if (a.kept != nullptr && tw % GS_TILE == 0 && tw < a.T && l.stores) st_state<V>(a.kept + (int64_t)(tw / GS_TILE) * a.B * a.D, h, l);
             T* yp = y + (int64_t)tw * a.D;
 #pragma unroll
             for (int s = 0; s < GS_S; ++s, yp += a.D) {
@@ -218,21 +227,21 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
                 }
                 if (stores_full) {
                     store_part<T, V>(yp, o, V);
-                } else if (tw + s < a.T && l.left > 0) {
+                } else if (tw + s < a.T && l.stores) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) o[v] = tw + s < l.len ? o[v] : 0.f;
-                    store_part<T, V>(yp, o, l.left);
+                    store_part<T, V>(yp, o, V);
                 }
             }
         }
     }
-    if (w != 0 || l.left <= 0) return;
+    if (w != 0 || !l.stores) return;
     if constexpr (SUM) {
         const int64_t n = (int64_t)a.B * a.D;
-        store_part<float, V>(a.maps + (2 * (int64_t)blockIdx.y) * n + l.ch, pA, l.left);
-        store_part<float, V>(a.maps + (2 * (int64_t)blockIdx.y + 1) * n + l.ch, c, l.left);
+        st_state<V>(a.maps + (2 * (int64_t)blockIdx.y) * n, pA, l);
+        st_state<V>(a.maps + (2 * (int64_t)blockIdx.y + 1) * n, c, l);
     } else if (a.hl != nullptr && (int)blockIdx.y == a.parts - 1) {
-        store_part<float, V>(a.hl + l.ch, c, l.left);
+        st_state<V>(a.hl, c, l);
     }
 }
 
@@ -253,13 +262,13 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
     float c[V], pA[V], hn[V];  // c: f_{t+1} dh_{t+1} behind the tile (dh_last behind the series); hn: state before the next tile
     Steps<T, V> xr, gr, dr;
     xr.zero(), dr.zero();
-    bool full = gs_full<V>(l, last + w * GS_S);
+    bool full = gs_full(l, last + w * GS_S);
     auto fetch = [&](int t0) {
         const int tw = t0 + w * GS_S;
-        gr.load(g, a.gt, tw, l.len, l, full);
-        if (a.dy != nullptr) dr.load(dy, a.dyt, tw, l.len, l, full);
+        gr.load(g, a.gt, tw, l, full);
+        if (a.dy != nullptr) dr.load(dy, a.dyt, tw, l, full);
         if constexpr (!SUM) {
-            xr.load(x, a.xt, tw, l.len, l, full);
+            xr.load(x, a.xt, tw, l, full);
             const float* from = t0 == 0 ? a.h0 : a.kept + (int64_t)(t0 / GS_TILE) * a.B * a.D;
 #pragma unroll
             for (int v = 0; v < V; ++v) hn[v] = 0.f;
@@ -287,16 +296,19 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                 if constexpr (!SUM) xs[s][v] = (float)xr.v[s].v[v];
                 ds[s][v] = (float)dr.v[s].v[v];
             }
-        if (!full) {  // (what is not read is 0)
+        if (!full) {  // steps behind the end hold the state, whatever was read
 #pragma unroll
             for (int s = 0; s < GS_S; ++s)
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (tw + s >= l.len) f[s][v] = 1.f, i[s][v] = 0.f;
+                    if (tw + s >= l.len) {
+                        f[s][v] = 1.f, i[s][v] = ds[s][v] = 0.f;
+                        if constexpr (!SUM) xs[s][v] = 0.f;
+                    }
         }
         const bool stores_full = full;
         if (t0 - W * GS_S >= t_lo) {
-            full = gs_full<V>(l, tw - W * GS_S);
+            full = gs_full(l, tw - W * GS_S);
             fetch(t0 - W * GS_S);
         }
 #pragma unroll
@@ -362,37 +374,67 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                 if (stores_full) {
                     if (a.dx != nullptr) store_part<T, V>(xp, ox, V);
                     if (a.dg != nullptr) store_part<T, V>(gp, og, V);
-                } else if (tw + s < a.T && l.left > 0) {
+                } else if (tw + s < a.T && l.stores) {
 #pragma unroll
                     for (int v = 0; v < V; ++v)
                         if (tw + s >= l.len) ox[v] = og[v] = 0.f;
-                    if (a.dx != nullptr) store_part<T, V>(xp, ox, l.left);
-                    if (a.dg != nullptr) store_part<T, V>(gp, og, l.left);
+                    if (a.dx != nullptr) store_part<T, V>(xp, ox, V);
+                    if (a.dg != nullptr) store_part<T, V>(gp, og, V);
                 }
             }
         }
     }
-    if (w != 0 || l.left <= 0) return;
+    if (w != 0 || !l.stores) return;
     if constexpr (SUM) {
         const int64_t n = (int64_t)a.B * a.D;
-        store_part<float, V>(a.maps + (2 * (int64_t)blockIdx.y) * n + l.ch, pA, l.left);
-        store_part<float, V>(a.maps + (2 * (int64_t)blockIdx.y + 1) * n + l.ch, c, l.left);
+        st_state<V>(a.maps + (2 * (int64_t)blockIdx.y) * n, pA, l);
+        st_state<V>(a.maps + (2 * (int64_t)blockIdx.y + 1) * n, c, l);
     } else if (a.dh0 != nullptr && blockIdx.y == 0) {
-        store_part<float, V>(a.dh0 + l.ch, c, l.left);
+        st_state<V>(a.dh0, c, l);
     }
+}
+
+// A few steps (serving: one): a lane walks its features' steps in turn.
+template <typename T, int V>
+__global__ __launch_bounds__(64) void gscan_step_k(const GsArgs a) {
+    const GsLane l = gs_lane<V>(a);
+    if (!l.stores) return;
+    const T* x = (const T*)a.x + (int64_t)l.b * a.xb + l.d;
+    const T* g = (const T*)a.g + (int64_t)l.b * a.gb + l.d;
+    T* y = (T*)a.y + (int64_t)l.b * a.T * a.D + l.d;
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = 0.f;
+    if (a.h0 != nullptr) ld_state<V>(h, a.h0, l);
+    for (int t = 0; t < a.T; ++t, y += a.D) {
+        float xs[V], gs[V], o[V];
+        const int tr = t < l.t_max ? t : l.t_max;
+        load_part<T, V>(xs, x + tr * a.xt, V);
+        load_part<T, V>(gs, g + tr * a.gt, V);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float f, i;
+            gate_pair(gs[v], f, i);
+            if (t < l.len) h[v] = fmaf(f, h[v], i * xs[v]);
+            o[v] = t < l.len ? h[v] : 0.f;
+        }
+        store_part<T, V>(y, o, V);
+    }
+    if (a.hl != nullptr) st_state<V>(a.hl, h, l);
 }
 
 int64_t gs_columns(int B, int D, int V) { return ceil_div64((int64_t)B * ((D + V - 1) / V), 64); }
 
-// What a launch looks like: V features a lane (8 bytes where there are channels enough, fewer until there are 256 columns of
-// workgroups), W waves a workgroup, parts of the time axis.
+// What a launch looks like: V features a lane (as many as leave 256 columns of workgroups; at most 8 bytes forward, 8 and 4 bytes
+// (fp32 and 16-bit types) backward, where more would not stay in registers; never more than D), W waves a workgroup, parts of the
+// time axis.
 struct GsPlan {
     int V, W, parts, part_steps;
 };
-GsPlan gs_plan(int B, int T, int D, int esize) {
+GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
     GsPlan p;
-    p.V = esize == 2 ? 4 : 2;
-    while (p.V > 1 && gs_columns(B, D, p.V) < 256) p.V >>= 1;
+    p.V = esize == 2 && fwd ? 4 : 2;
+    while (p.V > 1 && (p.V > D || gs_columns(B, D, p.V) < 256)) p.V >>= 1;
     const int64_t cols = gs_columns(B, D, p.V);
     p.W = T <= GS_S ? 1 : T <= 4 * GS_S ? 4 : cols >= 512 || T <= GS_TILE || p.V > 1 ? 8 : 16;
     const int64_t tile = p.W * GS_S, tiles = ceil_div64(T, tile);
@@ -415,7 +457,8 @@ int gs_launch(const GsArgs& a) {
             VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k (maps)" : "gscan_bwd_k (maps)");
         }
     }
-    if (FWD) gscan_fwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
+    if constexpr (FWD && W == 1) gscan_step_k<T, V><<<grid, dim3(64), 0, a.s>>>(a);
+    else if constexpr (FWD) gscan_fwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
     else gscan_bwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
     VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k" : "gscan_bwd_k");
     return VAE_OK;
@@ -423,7 +466,7 @@ int gs_launch(const GsArgs& a) {
 
 template <typename T, bool FWD>
 int gs_run(GsArgs& a) {
-    const GsPlan p = gs_plan(a.B, a.T, a.D, sizeof(T));
+    const GsPlan p = gs_plan(a.B, a.T, a.D, sizeof(T), FWD);
     a.parts = p.parts, a.part_steps = p.part_steps;
     if (a.parts > 1 && a.maps == nullptr) VAE_FAIL(VAE_EINVAL, "gated_scan: null workspace");
 #define VAE_GS(NV)                                                      \
@@ -435,7 +478,7 @@ int gs_run(GsArgs& a) {
     }
     VAE_GS(1)
     VAE_GS(2)
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && FWD) {
         VAE_GS(4)
     }
 #undef VAE_GS
@@ -458,7 +501,8 @@ extern "C" int64_t vae_gated_scan_kept_floats(int B, int T, int D) {
 
 extern "C" int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype) {
     if (B < 1 || T < 1 || D < 1 || vae_type_size(dtype) == 0) return 0;
-    const int p = gs_plan(B, T, D, vae_type_size(dtype)).parts;
+    const int f = gs_plan(B, T, D, vae_type_size(dtype), true).parts, b = gs_plan(B, T, D, vae_type_size(dtype), false).parts;
+    const int p = f > b ? f : b;  // (one size for both passes)
     return p > 1 ? 2 * (int64_t)p * B * D : 0;
 }
 
