@@ -23,7 +23,7 @@ def _dtype(what, t):
 
 
 def _same(what, t, name, shape, dtypes, device):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype not in dtypes:
         raise L.VaeAmdError(f"{what}: {name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
@@ -72,45 +72,40 @@ def _needs_grad(*ts):
 def _norm_forward(x, weight, bias, eps, save):
     C = x.shape[-1]
     xr, rows, ld = _rows(x, C)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stat = torch.empty((2, rows), dtype=torch.float32, device=x.device) if save else None
+    y = torch.empty_like(xr, memory_format=torch.contiguous_format)
+    stat = xr.new_empty((2, rows), dtype=torch.float32) if save else None
     w = weight if weight is not None else bias
+    wtype = _TYPES[w.dtype] if w is not None else L.T_F32
     if rows:
         sp = stat.data_ptr() if save else None
         _call(L.lib().vae_layer_norm_forward, "vae_layer_norm_forward", x.device, xr.data_ptr(), ld, _p(weight), _p(bias),
-              y.data_ptr(), C, sp, sp + 4 * rows if save else None, rows, C, eps, _TYPES[x.dtype],
-              _TYPES[w.dtype] if w is not None else L.T_F32)
-    return y, xr, stat
+              y.data_ptr(), C, sp, sp + 4 * rows if save else None, rows, C, eps, _TYPES[x.dtype], wtype)
+    return y, xr, rows, ld, stat, wtype
 
 
 class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, xr, stat = _norm_forward(x, weight, bias, eps, True)
+        y, xr, rows, ld, stat, wtype = _norm_forward(x, weight, bias, eps, True)
         ctx.save_for_backward(xr, weight, bias, stat)
-        ctx.shape = x.shape
+        ctx.geom = rows, x.shape[-1], ld, wtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xr, weight, bias, stat = ctx.saved_tensors
-        C = ctx.shape[-1]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(ctx.shape, dtype=xr.dtype, device=xr.device) if need_x else None
+        rows, C, ldx, wtype = ctx.geom
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = torch.empty_like(xr, memory_format=torch.contiguous_format) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        _, rows, ldx = _rows(xr, C)
-        dyr, _, lddy = _rows(dy, C)
-        ws = None
-        if need_w or need_b:
-            ws = torch.empty(L.lib().vae_layer_norm_workspace_floats(rows, C), dtype=torch.float32, device=xr.device)
-        w = weight if weight is not None else bias
+        dy, _, lddy = _rows(dy, C)
+        lib = L.lib()
+        ws = xr.new_empty(lib.vae_layer_norm_workspace_floats(rows, C), dtype=torch.float32) if need_w or need_b else None
         sp = stat.data_ptr()
-        if C:
-            _call(L.lib().vae_layer_norm_backward, "vae_layer_norm_backward", xr.device, dyr.data_ptr(), lddy, xr.data_ptr(),
-                  ldx, _p(weight), sp, sp + 4 * rows, _p(dx), C, _p(dw), _p(db), _p(ws), rows, C, _TYPES[xr.dtype],
-                  _TYPES[w.dtype] if w is not None else L.T_F32)
+        _call(lib.vae_layer_norm_backward, "vae_layer_norm_backward", xr.device, dy.data_ptr(), lddy, xr.data_ptr(), ldx, _p(weight),
+              sp, sp + 4 * rows, _p(dx), C, _p(dw), _p(db), _p(ws), rows, C, _TYPES[xr.dtype], wtype)
         return dx, dw, db, None
 
 
@@ -143,48 +138,44 @@ def _linear_forward(x, weight, bias, act, slope, residual, save):
     N, K = weight.shape
     xr, M, ldx = _rows(x, K)
     wr, _, ldw = _rows(weight, K)
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    y = xr.new_empty(x.shape[:-1] + (N,))
     code = _TYPES[x.dtype]
     aux = None
     if M:
         rr, ldr = None, 0
         if residual is not None:
             rr, _, ldr = _rows(residual, N)
+        lib = L.lib()
         if save and act != L.ACT_NONE:
-            aux = torch.empty(L.lib().vae_dense_aux_bytes(M, N, act, code), dtype=torch.uint8, device=x.device)
-        _call(L.lib().vae_dense_forward, "vae_dense_forward", x.device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr),
-              ldr, y.data_ptr(), N, _p(aux), M, N, K, act, slope, code)
-    return y, xr, wr, aux
+            aux = xr.new_empty(lib.vae_dense_aux_bytes(M, N, act, code), dtype=torch.uint8)
+        _call(lib.vae_dense_forward, "vae_dense_forward", x.device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr), ldr,
+              y.data_ptr(), N, _p(aux), M, N, K, act, slope, code)
+    return y, xr, wr, aux, (M, N, K, ldx, ldw, act, slope, code)
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, slope):
-        y, xr, wr, aux = _linear_forward(x, weight, bias, act, slope, residual, True)
+        y, xr, wr, aux, ctx.geom = _linear_forward(x, weight, bias, act, slope, residual, True)
         ctx.save_for_backward(xr, wr, aux)
-        ctx.shape, ctx.act, ctx.slope = x.shape, act, slope
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xr, wr, aux = ctx.saved_tensors
-        N, K = wr.shape
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        M = dy.numel() // N
-        dev, dt, code = xr.device, xr.dtype, _TYPES[xr.dtype]
-        alloc = torch.empty if M else torch.zeros
-        dx = alloc(ctx.shape, dtype=dt, device=dev) if need_x else None
-        dw = alloc((N, K), dtype=dt, device=dev) if need_w else None
-        db = alloc((N,), dtype=dt, device=dev) if need_b else None
+        M, N, K, ldx, ldw, act, slope, code = ctx.geom
+        need_x, need_w, need_b, need_r, _, _ = ctx.needs_input_grad
+        like = torch.empty_like if M else torch.zeros_like
+        dx = like(xr, memory_format=torch.contiguous_format) if need_x else None
+        dw = like(wr, memory_format=torch.contiguous_format) if need_w else None
+        db = (xr.new_empty if M else xr.new_zeros)((N,)) if need_b else None
         if M and (need_x or need_w or need_b):
-            _, _, ldx = _rows(xr, K)
-            _, _, ldw = _rows(wr, K)
             dyr, _, lddy = _rows(dy, N)
             lib = L.lib()
-            ws = torch.empty(lib.vae_dense_workspace_floats(M, N, K, ctx.act, code), dtype=torch.float32, device=dev)
-            _call(lib.vae_dense_backward, "vae_dense_backward", dev, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, wr.data_ptr(), ldw,
-                  _p(aux), _p(dx), _p(dw), _p(db), ws.data_ptr(), M, N, K, ctx.act, ctx.slope, code)
+            ws = xr.new_empty(lib.vae_dense_workspace_floats(M, N, K, act, code), dtype=torch.float32)
+            _call(lib.vae_dense_backward, "vae_dense_backward", xr.device, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, wr.data_ptr(),
+                  ldw, _p(aux), _p(dx), _p(dw), _p(db), ws.data_ptr(), M, N, K, act, slope, code)
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -226,15 +217,15 @@ def _scan_forward(x, gate, h0, lengths, save):
     dev = x.device
     xs, xb, xt = _steps(x)
     gs, gb, gt = _steps(gate)
-    y = torch.empty((B, T, D), dtype=x.dtype, device=dev)
-    hl = torch.empty((B, D), dtype=torch.float32, device=dev)
+    y = torch.empty_like(xs, memory_format=torch.contiguous_format)
+    hl = xs.new_empty((B, D), dtype=torch.float32)
     kept = None
     lib, code = L.lib(), _TYPES[x.dtype]
     n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    ws = xs.new_empty(n, dtype=torch.float32) if n else None
     if save:
         n = lib.vae_gated_scan_kept_floats(B, T, D)
-        kept = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+        kept = xs.new_empty(n, dtype=torch.float32) if n else None
     _call(lib.vae_gated_scan_forward, "vae_gated_scan_forward", dev, xs.data_ptr(), xb, xt, gs.data_ptr(), gb, gt, _p(h0),
           _p(lengths), y.data_ptr(), hl.data_ptr(), _p(kept), _p(ws), B, T, D, code)
     return y, hl, xs, gs, kept
@@ -254,12 +245,12 @@ class _ScanFn(torch.autograd.Function):
         xs, gs, h0, lengths, kept = ctx.saved_tensors
         B, T, D = xs.shape
         dev = xs.device
-        need_x, need_g, need_h = ctx.needs_input_grad[:3]
+        need_x, need_g, need_h, _ = ctx.needs_input_grad
         if dy is None and dhl is None:
             return None, None, None, None
-        dx = torch.empty((B, T, D), dtype=xs.dtype, device=dev) if need_x else None
-        dg = torch.empty((B, T, D), dtype=xs.dtype, device=dev) if need_g else None
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if need_h else None
+        dx = torch.empty_like(xs, memory_format=torch.contiguous_format) if need_x else None
+        dg = torch.empty_like(xs, memory_format=torch.contiguous_format) if need_g else None
+        dh0 = torch.empty_like(h0) if need_h else None
         db = dt = 0
         if dy is not None:
             dy, db, dt = _steps(dy)
@@ -267,7 +258,7 @@ class _ScanFn(torch.autograd.Function):
             dhl = dhl.contiguous()
         lib, code = L.lib(), _TYPES[xs.dtype]
         n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
-        ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+        ws = xs.new_empty(n, dtype=torch.float32) if n else None
         _call(lib.vae_gated_scan_backward, "vae_gated_scan_backward", dev, _p(dy), db, dt, _p(dhl), xs.data_ptr(), xs.stride(0),
               xs.stride(1), gs.data_ptr(), gs.stride(0), gs.stride(1), _p(h0), _p(lengths), _p(kept), _p(dx), _p(dg), _p(dh0),
               _p(ws), B, T, D, code)
