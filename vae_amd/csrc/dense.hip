@@ -17,7 +17,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // What the derivative needs of p: one byte that says p > 0 for the leaky ReLU; else p itself, in fp16 where the tensors are bf16
 // (three more bits than their own type: the rounding then adds nothing to what the gradients' own type loses; act' is flat
-// beyond fp16's range, so p is clamped to it) and in fp32 where they are fp16 or fp32.
+// beyond fp16's range, so what becomes infinite is read as its largest number) and in fp32 where they are fp16 or fp32.
 enum { AUX_NONE = 0, AUX_U8 = 1, AUX_F16 = 2, AUX_F32 = 4 };
 inline int aux_kind(int act, int dtype) {
     if (act == VAE_ACT_NONE) return AUX_NONE;
@@ -27,9 +27,10 @@ inline int aux_kind(int act, int dtype) {
 
 // Normal distribution function and exp(-p^2/2): erfc by Abramowitz & Stegun 7.1.26, (a1 t + .. + a5 t^5) exp(-x^2) with
 // t = 1 / (1 + 0.3275911 x), x = |p| / sqrt 2, off by at most 1.5e-7 (the function half of that); no branches.
+template <bool FAST>
 __device__ __forceinline__ float normal_cdf(float p, float& e) {
     const float x = fabsf(p) * 0.70710678f;
-    e = exp_acc(-x * x);
+    e = FAST ? exp_fast(-x * x) : exp_acc(-x * x);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
     float u = fmaf(t, 1.061405429f, -1.453152027f);
     u = fmaf(t, u, 1.421413741f);
@@ -38,7 +39,8 @@ __device__ __forceinline__ float normal_cdf(float p, float& e) {
     return p < 0.f ? u : 1.f - u;
 }
 
-// act and act' of 8 values: the switch stands outside the loop over them
+// act and act' of 8 values: the switch stands outside the loop over them.  FAST: the results are rounded to 16 bits.
+template <bool FAST>
 __device__ __forceinline__ void dense_act8(float (&v)[8], int act, float slope) {
     float f, i;
     switch (act) {
@@ -48,35 +50,36 @@ __device__ __forceinline__ void dense_act8(float (&v)[8], int act, float slope) 
             break;
         case VAE_ACT_SIGMOID:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate_pair(v[e], f, i), v[e] = f;
+            for (int e = 0; e < 8; ++e) gate_pair<FAST>(v[e], f, i), v[e] = f;
             break;
         case VAE_ACT_GELU:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= normal_cdf(v[e], f);
+            for (int e = 0; e < 8; ++e) v[e] *= normal_cdf<FAST>(v[e], f);
             break;
         case VAE_ACT_SILU:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate_pair(v[e], f, i), v[e] *= f;
+            for (int e = 0; e < 8; ++e) gate_pair<FAST>(v[e], f, i), v[e] *= f;
             break;
     }
 }
+template <bool FAST>
 __device__ __forceinline__ void dense_act_grad8(float (&d)[8], const float (&p)[8], int act) {  // d *= act'(p)
     float f, i;
     switch (act) {
         case VAE_ACT_SIGMOID:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate_pair(p[e], f, i), d[e] *= f * i;
+            for (int e = 0; e < 8; ++e) gate_pair<FAST>(p[e], f, i), d[e] *= f * i;
             break;
         case VAE_ACT_GELU:
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float c = normal_cdf(p[e], f);
+                const float c = normal_cdf<FAST>(p[e], f);
                 d[e] *= fmaf(p[e] * f, 0.39894228f, c);
             }
             break;
         case VAE_ACT_SILU:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate_pair(p[e], f, i), d[e] *= f * fmaf(p[e], i, 1.f);
+            for (int e = 0; e < 8; ++e) gate_pair<FAST>(p[e], f, i), d[e] *= f * fmaf(p[e], i, 1.f);
             break;
     }
 }
@@ -140,10 +143,11 @@ template <typename T, int R, bool RC, int NT>
 struct Stage {
     static constexpr int V = 16 / sizeof(T), N = R * 8 / NT;
     Pack<T, V> r[N];
-    // A tile inside the operand is loaded without a test an element.  (k contiguous: rows behind the last are read as the last one;
-    // what they give is not stored.)
-    __device__ __forceinline__ void load(const T* p, int64_t ld, int r0, int rows, int k0, int kend, int tid) {
-        if (k0 + BK<T>() <= kend && (!RC || r0 + R <= rows)) {
+    // A tile inside the operand is loaded without a test an element.  What rows behind the last give is not stored, so they may hold
+    // anything: with k contiguous they are read as the last one, else the loads run on into the next row of k, which is there for
+    // all k but the operand's last (k_all: its number of k).
+    __device__ __forceinline__ void load(const T* p, int64_t ld, int r0, int rows, int k0, int kend, int k_all, int tid) {
+        if (k0 + BK<T>() <= kend && (!RC || r0 + R <= rows || (ld >= R && k0 + BK<T>() < k_all))) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const int c = tid + j * NT;
@@ -219,13 +223,7 @@ __device__ __forceinline__ void aux_store8(void* aux, int64_t at, const float (&
             for (int e = 0; e < 8; ++e)
                 if (e < left) q[e] = o.v[e];
     } else if (kind == AUX_F16) {
-        float c[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            c[e] = p[e] > 65504.f ? 65504.f : p[e];  // (a NaN passes)
-            c[e] = c[e] < -65504.f ? -65504.f : c[e];
-        }
-        store_part<f16_t, 8>((f16_t*)aux + at, c, left);
+        store_part<f16_t, 8>((f16_t*)aux + at, p, left);  // (beyond fp16: infinity)
     } else if (kind == AUX_F32) {
         store_part<float, 8>((float*)aux + at, p, left);
     }
@@ -281,7 +279,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += bias[e];
             if (g.aux != nullptr) aux_store8(g.aux, m * g.N + n, v, g.auxk, left);
-            dense_act8(v, g.act, g.slope);
+            dense_act8<sizeof(T) == 2>(v, g.act, g.slope);
             if (has_res) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += (float)r.v[e];
@@ -328,8 +326,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
     for (int d = 0; d < AHEAD; ++d) {
         const int k = k_lo + d * BK<T>();
         if (k >= k_hi) break;
-        sa[d].load((const T*)g.a, g.lda, m0, g.M, k, k_hi, tid);
-        sb[d].load((const T*)g.b, g.ldb, n0, g.N, k, k_hi, tid);
+        sa[d].load((const T*)g.a, g.lda, m0, g.M, k, k_hi, g.K, tid);
+        sb[d].load((const T*)g.b, g.ldb, n0, g.N, k, k_hi, g.K, tid);
     }
     int cur = 0;
     for (int kk = k_lo; kk < k_hi; kk += AHEAD * BK<T>())
@@ -343,8 +341,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
             sb[d].put(pb, tid);
             const int kn = k0 + AHEAD * BK<T>();
             if (kn < k_hi) {
-                sa[d].load((const T*)g.a, g.lda, m0, g.M, kn, k_hi, tid);
-                sb[d].load((const T*)g.b, g.ldb, n0, g.N, kn, k_hi, tid);
+                sa[d].load((const T*)g.a, g.lda, m0, g.M, kn, k_hi, g.K, tid);
+                sb[d].load((const T*)g.b, g.ldb, n0, g.N, kn, k_hi, g.K, tid);
             }
             lds_barrier();  // (two buffers: the writes of the next tile go to the one that no wave reads any more)
 #pragma unroll
@@ -563,7 +561,7 @@ __global__ __launch_bounds__(MF == 4 ? 512 : 1024) void dense_rows_k(const GemmA
         for (int k = 0; k < nw; ++k) v[0] += red[k][m >> 4][m & 15][o & 15];
         if (g.bias != nullptr) v[0] += (float)((const T*)g.bias)[n];
         if (g.aux != nullptr) aux_store8(g.aux, (int64_t)m * g.N + n, v, g.auxk, 1);
-        dense_act8(v, g.act, g.slope);
+        dense_act8<sizeof(T) == 2>(v, g.act, g.slope);
         if (g.res != nullptr) v[0] += (float)((const T*)g.res)[(int64_t)m * g.ldr + n];
         ((T*)g.c)[(int64_t)m * g.ldc + n] = (T)v[0];
     }
@@ -625,7 +623,12 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
                 } else {
                     if (auxk == AUX_F16) load_part<f16_t, 8>(p, (const f16_t*)aux + at, left, N >= 8);
                     else load_part<float, 8>(p, (const float*)aux + at, left);
-                    dense_act_grad8(v, p, act);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {  // act' is flat out there, and infinity would make p exp(-p^2/2) a NaN (a NaN passes)
+                        p[e] = p[e] > 65504.f ? 65504.f : p[e];
+                        p[e] = p[e] < -65504.f ? -65504.f : p[e];
+                    }
+                    dense_act_grad8<sizeof(T) == 2>(v, p, act);
                 }
                 store_part<T, 8>(dp + m * ldp + n, v, left);
             }

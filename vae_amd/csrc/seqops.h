@@ -78,12 +78,16 @@ __device__ __forceinline__ float exp_acc(float x) {
     return fmaf(e, lost * 0.69314718f, e);
 }
 
+// ... and one of |x| 2^-24, in two instructions, for results that are rounded to 16 bits
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
 // f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1).  The clamp
 // keeps exp finite; a NaN passes it.
+template <bool FAST = false>
 __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
     g = g > 87.f ? 87.f : g;
     g = g < -87.f ? -87.f : g;
-    const float e = exp_acc(-g);
+    const float e = FAST ? exp_fast(-g) : exp_acc(-g);
     const float r = __builtin_amdgcn_rcpf(1.f + e);  // (one unit in the last place)
     f = r;
     i = e * r;
