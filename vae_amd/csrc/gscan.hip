@@ -19,6 +19,7 @@
 namespace {
 
 constexpr int GS_S = 8;               // steps a wave holds
+constexpr int gs_steps(int W) { return W == 16 ? 16 : GS_S; }  // ... forward, in workgroups that have a CU each: twice the loads in flight
 constexpr int GS_TILE = 64;           // steps between two kept states
 constexpr int GS_MAX_PARTS = 64;
 
@@ -114,31 +115,32 @@ __device__ __forceinline__ void enter_part(float (&c)[V], const float* first, co
 }
 
 // A wave's S steps of one tensor as they lie in memory; steps behind the sequence's end are read as its last one and not used.
-template <typename T, int V>
+template <typename T, int V, int S>
 struct Steps {
-    Pack<T, V> v[GS_S];
+    Pack<T, V> v[S];
     __device__ __forceinline__ void load(const T* p, int64_t st, int t, const GsLane& l, bool full) {
         if (full) {
             const T* q = p + (int64_t)t * st;
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s, q += st) v[s] = *reinterpret_cast<const Pack<T, V>*>(q);
+            for (int s = 0; s < S; ++s, q += st) v[s] = *reinterpret_cast<const Pack<T, V>*>(q);
         } else {
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s) v[s] = *reinterpret_cast<const Pack<T, V>*>(p + (int64_t)(t + s < l.t_max ? t + s : l.t_max) * st);
+            for (int s = 0; s < S; ++s) v[s] = *reinterpret_cast<const Pack<T, V>*>(p + (int64_t)(t + s < l.t_max ? t + s : l.t_max) * st);
         }
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int s = 0; s < GS_S; ++s)
+        for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int i = 0; i < V; ++i) v[s].v[i] = (T)0.f;
     }
 };
 // Do all lanes of the wave have the steps t .. t + S - 1 in their sequences, and store what they compute?
-__device__ __forceinline__ bool gs_full(const GsLane& l, int t) { return __all(l.stores && t + GS_S <= l.len); }
+template <int S>
+__device__ __forceinline__ bool gs_full(const GsLane& l, int t) { return __all(l.stores && t + S <= l.len); }
 
 // SUM: leave the part's map only.
-template <typename T, int V, int W, bool SUM>
+template <typename T, int V, int W, int S, bool SUM>
 __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
     __shared__ float lds[2][W * 2 * 64 * V];
     const GsLane l = gs_lane<V>(a);
@@ -149,10 +151,10 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
     const int t_lo = (int)blockIdx.y * a.part_steps;
     const int t_hi = a.T - t_lo < a.part_steps ? a.T : t_lo + a.part_steps;
     float c[V], pA[V];
-    Steps<T, V> xr, gr;
-    bool full = gs_full(l, t_lo + w * GS_S);
-    xr.load(x, a.xt, t_lo + w * GS_S, l, full);
-    gr.load(g, a.gt, t_lo + w * GS_S, l, full);
+    Steps<T, V, S> xr, gr;
+    bool full = gs_full<S>(l, t_lo + w * S);
+    xr.load(x, a.xt, t_lo + w * S, l, full);
+    gr.load(g, a.gt, t_lo + w * S, l, full);
     if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = 0.f, pA[v] = 1.f;
@@ -160,34 +162,34 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
         enter_part<V, W, false>(c, a.h0, a, l, lds[0]);
     }
     int flip = 0;
-    for (int t0 = t_lo; t0 < t_hi; t0 += W * GS_S, flip ^= 1) {
-        const int tw = t0 + w * GS_S;
-        float f[GS_S][V], b[GS_S][V], A[V], H[V];
+    for (int t0 = t_lo; t0 < t_hi; t0 += W * S, flip ^= 1) {
+        const int tw = t0 + w * S;
+        float f[S][V], b[S][V], A[V], H[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f;
 #pragma unroll
-        for (int s = 0; s < GS_S; ++s)
+        for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float i;
-                gate_pair((float)gr.v[s].v[v], f[s][v], i);
+                gate_pair<sizeof(T) == 2>((float)gr.v[s].v[v], f[s][v], i);
                 b[s][v] = i * (float)xr.v[s].v[v];
             }
         if (!full) {  // steps behind the end hold the state
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s)
+            for (int s = 0; s < S; ++s)
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     if (tw + s >= l.len) f[s][v] = 1.f, b[s][v] = 0.f;
         }
         const bool stores_full = full;
-        if (t0 + W * GS_S < t_hi) {  // the next tile's loads run while this one is worked on
-            full = gs_full(l, tw + W * GS_S);
-            xr.load(x, a.xt, tw + W * GS_S, l, full);
-            gr.load(g, a.gt, tw + W * GS_S, l, full);
+        if (t0 + W * S < t_hi) {  // the next tile's loads run while this one is worked on
+            full = gs_full<S>(l, tw + W * S);
+            xr.load(x, a.xt, tw + W * S, l, full);
+            gr.load(g, a.gt, tw + W * S, l, full);
         }
 #pragma unroll
-        for (int s = 0; s < GS_S; ++s)
+        for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 A[v] *= f[s][v];
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(W * 64) void gscan_fwd_k(const GsArgs a) {
             if (a.kept != nullptr && tw % GS_TILE == 0 && tw < a.T && l.stores) st_state<V>(a.kept + (int64_t)(tw / GS_TILE) * a.B * a.D, h, l);
             T* yp = y + (int64_t)tw * a.D;
 #pragma unroll
-            for (int s = 0; s < GS_S; ++s, yp += a.D) {
+            for (int s = 0; s < S; ++s, yp += a.D) {
                 float o[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -260,9 +262,9 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
     const int t_hi = a.T - t_lo < a.part_steps ? a.T : t_lo + a.part_steps;
     const int last = t_lo + (t_hi - 1 - t_lo) / (W * GS_S) * (W * GS_S);
     float c[V], pA[V], hn[V];  // c: f_{t+1} dh_{t+1} behind the tile (dh_last behind the series); hn: state before the next tile
-    Steps<T, V> xr, gr, dr;
+    Steps<T, V, GS_S> xr, gr, dr;
     xr.zero(), dr.zero();
-    bool full = gs_full(l, last + w * GS_S);
+    bool full = gs_full<GS_S>(l, last + w * GS_S);
     auto fetch = [&](int t0) {
         const int tw = t0 + w * GS_S;
         gr.load(g, a.gt, tw, l, full);
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
         for (int s = 0; s < GS_S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gate_pair((float)gr.v[s].v[v], f[s][v], i[s][v]);
+                gate_pair<sizeof(T) == 2>((float)gr.v[s].v[v], f[s][v], i[s][v]);
                 if constexpr (!SUM) xs[s][v] = (float)xr.v[s].v[v];
                 ds[s][v] = (float)dr.v[s].v[v];
             }
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
         }
         const bool stores_full = full;
         if (t0 - W * GS_S >= t_lo) {
-            full = gs_full(l, tw - W * GS_S);
+            full = gs_full<GS_S>(l, tw - W * GS_S);
             fetch(t0 - W * GS_S);
         }
 #pragma unroll
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(64) void gscan_step_k(const GsArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float f, i;
-            gate_pair(gs[v], f, i);
+            gate_pair<sizeof(T) == 2>(gs[v], f, i);
             if (t < l.len) h[v] = fmaf(f, h[v], i * xs[v]);
             o[v] = t < l.len ? h[v] : 0.f;
         }
@@ -437,7 +439,7 @@ GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
     while (p.V > 1 && (p.V > D || gs_columns(B, D, p.V) < 256)) p.V >>= 1;
     const int64_t cols = gs_columns(B, D, p.V);
     p.W = T <= GS_S ? 1 : T <= 4 * GS_S ? 4 : cols >= 512 || T <= GS_TILE || p.V > 1 ? 8 : 16;
-    const int64_t tile = p.W * GS_S, tiles = ceil_div64(T, tile);
+    const int64_t tile = p.W * (fwd ? gs_steps(p.W) : GS_S), tiles = ceil_div64(T, tile);
     int64_t n = cols >= 192 ? 1 : ceil_div64(512, cols);
     if (n > GS_MAX_PARTS) n = GS_MAX_PARTS;
     if (n > tiles) n = tiles;
@@ -452,13 +454,13 @@ int gs_launch(const GsArgs& a) {
     const dim3 grid((unsigned)gs_columns(a.B, a.D, V), a.parts);
     if constexpr (W >= 8) {
         if (a.parts > 1) {
-            if (FWD) gscan_fwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
+            if (FWD) gscan_fwd_k<T, V, W, gs_steps(W), true><<<grid, dim3(W * 64), 0, a.s>>>(a);
             else gscan_bwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
             VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k (maps)" : "gscan_bwd_k (maps)");
         }
     }
     if constexpr (FWD && W == 1) gscan_step_k<T, V><<<grid, dim3(64), 0, a.s>>>(a);
-    else if constexpr (FWD) gscan_fwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
+    else if constexpr (FWD) gscan_fwd_k<T, V, W, gs_steps(W), false><<<grid, dim3(W * 64), 0, a.s>>>(a);
     else gscan_bwd_k<T, V, W, false><<<grid, dim3(W * 64), 0, a.s>>>(a);
     VAE_LAUNCH_CHECK(FWD ? "gscan_fwd_k" : "gscan_bwd_k");
     return VAE_OK;

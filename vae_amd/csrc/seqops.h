@@ -81,16 +81,22 @@ __device__ __forceinline__ float exp_acc(float x) {
 // ... and one of |x| 2^-24, in two instructions, for results that are rounded to 16 bits
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
-// f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1).  The clamp
-// keeps exp finite; a NaN passes it.
+// f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1); infinite gates give
+// 0 and 1, a NaN passes.  FAST, for 16-bit tensors: exp may be off by |g| 2^-24; f then is by (1 - f) of that, so over the
+// 1 / (1 - f) steps that a recurrence remembers it adds up to no more.
 template <bool FAST = false>
 __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
-    g = g > 87.f ? 87.f : g;
-    g = g < -87.f ? -87.f : g;
-    const float e = FAST ? exp_fast(-g) : exp_acc(-g);
-    const float r = __builtin_amdgcn_rcpf(1.f + e);  // (one unit in the last place)
-    f = r;
-    i = e * r;
+    if constexpr (FAST) {
+        const float e = exp_fast(-g);
+        f = __builtin_amdgcn_rcpf(1.f + e);
+        i = e > 1e30f ? 1.f : e * f;  // (where e is infinite)
+    } else {
+        g = g > 87.f ? 87.f : g;  // (keeps exp_acc finite)
+        g = g < -87.f ? -87.f : g;
+        const float e = exp_acc(-g);
+        f = __builtin_amdgcn_rcpf(1.f + e);  // (one unit in the last place)
+        i = e * f;
+    }
 }
 
 // Column sums of `rows` rows of n partial sums, in a fixed order: 64 columns a workgroup, 16 waves that take every 16th row.
