@@ -15,20 +15,25 @@ _TYPES = {torch.float32: L.T_F32, torch.bfloat16: L.T_BF16, torch.float16: L.T_F
 _ACTS = {"none": L.ACT_NONE, "leaky": L.ACT_LEAKY, "sigmoid": L.ACT_SIGMOID, "gelu": L.ACT_GELU, "silu": L.ACT_SILU}
 
 
-def _dtype(what, t):
-    try:
-        return _TYPES[t.dtype]
-    except KeyError:
-        raise L.VaeAmdError(f"{what}: fp32, bf16 or fp16 tensors (got {t.dtype})") from None
+def _begin(what, x):
+    """Checks of the first tensor: (device, VAE_T_* of its type)."""
+    device = x.device
+    if device.index not in L._device_ok:
+        L.require_device(x)
+    code = _TYPES.get(x.dtype)
+    if code is None:
+        raise L.VaeAmdError(f"{what}: fp32, bf16 or fp16 tensors (got {x.dtype})")
+    return device, code
 
 
 def _same(what, t, name, shape, dtypes, device):
+    if t.shape == shape and t.dtype in dtypes and t.device == device:
+        return
     if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype not in dtypes:
         raise L.VaeAmdError(f"{what}: {name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if t.device != device:
-        raise L.VaeAmdError(f"{what}: {name} is on {t.device}, the input on {device}")
+    raise L.VaeAmdError(f"{what}: {name} is on {t.device}, the input on {device}")
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (torch.cuda.current_stream() takes 15 us on the autograd thread)
@@ -53,7 +58,7 @@ def _p(t):
 def _rows(t, cols):
     """t as rows of `cols` contiguous elements at one stride: (tensor that owns the memory, rows, stride); copies where the
     strides are others."""
-    rows = t.numel() // cols if cols else 0
+    rows = t.numel() // cols
     if t.is_contiguous():
         return t, rows, cols
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
@@ -69,34 +74,37 @@ def _needs_grad(*ts):
 
 
 # ------------------------------------------------------------------------------------------------ layer norm
-def _norm_forward(x, weight, bias, eps, save):
+def _norm_forward(x, weight, bias, eps, device, code, save):
     C = x.shape[-1]
     xr, rows, ld = _rows(x, C)
     y = torch.empty_like(xr, memory_format=torch.contiguous_format)
-    stat = xr.new_empty((2, rows), dtype=torch.float32) if save else None
     w = weight if weight is not None else bias
     wtype = _TYPES[w.dtype] if w is not None else L.T_F32
+    stat = mean = rstd = None
+    if save:
+        stat = xr.new_empty((2, rows), dtype=torch.float32)
+        mean = stat.data_ptr()
+        rstd = mean + 4 * rows
     if rows:
-        sp = stat.data_ptr() if save else None
-        _call(L.lib().vae_layer_norm_forward, "vae_layer_norm_forward", x.device, xr.data_ptr(), ld, _p(weight), _p(bias),
-              y.data_ptr(), C, sp, sp + 4 * rows if save else None, rows, C, eps, _TYPES[x.dtype], wtype)
+        _call(L.lib().vae_layer_norm_forward, "vae_layer_norm_forward", device, xr.data_ptr(), ld, _p(weight), _p(bias), y.data_ptr(),
+              C, mean, rstd, rows, C, eps, code, wtype)
     return y, xr, rows, ld, stat, wtype
 
 
 class _NormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, xr, rows, ld, stat, wtype = _norm_forward(x, weight, bias, eps, True)
+    def forward(ctx, x, weight, bias, eps, device, code):
+        y, xr, rows, ld, stat, wtype = _norm_forward(x, weight, bias, eps, device, code, True)
         ctx.save_for_backward(xr, weight, bias, stat)
-        ctx.geom = rows, x.shape[-1], ld, wtype
+        ctx.geom = rows, x.shape[-1], ld, device, code, wtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xr, weight, bias, stat = ctx.saved_tensors
-        rows, C, ldx, wtype = ctx.geom
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        rows, C, ldx, device, code, wtype = ctx.geom
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty_like(xr, memory_format=torch.contiguous_format) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
@@ -104,9 +112,9 @@ class _NormFn(torch.autograd.Function):
         lib = L.lib()
         ws = xr.new_empty(lib.vae_layer_norm_workspace_floats(rows, C), dtype=torch.float32) if need_w or need_b else None
         sp = stat.data_ptr()
-        _call(lib.vae_layer_norm_backward, "vae_layer_norm_backward", xr.device, dy.data_ptr(), lddy, xr.data_ptr(), ldx, _p(weight),
-              sp, sp + 4 * rows, _p(dx), C, _p(dw), _p(db), _p(ws), rows, C, _TYPES[xr.dtype], wtype)
-        return dx, dw, db, None
+        _call(lib.vae_layer_norm_backward, "vae_layer_norm_backward", device, dy.data_ptr(), lddy, xr.data_ptr(), ldx, _p(weight),
+              sp, sp + 4 * rows, _p(dx), C, _p(dw), _p(db), _p(ws), rows, C, code, wtype)
+        return dx, dw, db, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -114,32 +122,29 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     x (..., C); weight, bias (C) or None, fp32 or of x's type (both of one type).  Rows may lie at any stride.  The gradients of
     weight and bias are sums over all rows in fp32, added in a fixed order."""
-    L.require_device(x)
-    _dtype("layer_norm", x)
+    device, code = _begin("layer_norm", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: input of shape {tuple(x.shape)}")
-    kinds = (torch.float32, x.dtype)
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _same("layer_norm", t, name, x.shape[-1:], kinds, x.device)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise L.VaeAmdError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    shape, kinds = x.shape[-1:], (torch.float32, x.dtype)
+    if weight is not None:
+        _same("layer_norm", weight, "weight", shape, kinds, device)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    if bias is not None:
+        _same("layer_norm", bias, "bias", shape, kinds if weight is None else (weight.dtype,), device)
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     if _needs_grad(x, weight, bias):
-        return _NormFn.apply(x, weight, bias, float(eps))
-    return _norm_forward(x, weight, bias, float(eps), False)[0]
+        return _NormFn.apply(x, weight, bias, float(eps), device, code)
+    return _norm_forward(x, weight, bias, float(eps), device, code, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------- linear
-def _linear_forward(x, weight, bias, act, slope, residual, save):
+def _linear_forward(x, weight, bias, act, slope, residual, device, code, save):
     N, K = weight.shape
     xr, M, ldx = _rows(x, K)
     wr, _, ldw = _rows(weight, K)
     y = xr.new_empty(x.shape[:-1] + (N,))
-    code = _TYPES[x.dtype]
     aux = None
     if M:
         rr, ldr = None, 0
@@ -148,15 +153,15 @@ def _linear_forward(x, weight, bias, act, slope, residual, save):
         lib = L.lib()
         if save and act != L.ACT_NONE:
             aux = xr.new_empty(lib.vae_dense_aux_bytes(M, N, act, code), dtype=torch.uint8)
-        _call(lib.vae_dense_forward, "vae_dense_forward", x.device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr), ldr,
+        _call(lib.vae_dense_forward, "vae_dense_forward", device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr), ldr,
               y.data_ptr(), N, _p(aux), M, N, K, act, slope, code)
-    return y, xr, wr, aux, (M, N, K, ldx, ldw, act, slope, code)
+    return y, xr, wr, aux, (M, N, K, ldx, ldw, act, slope, device, code)
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, slope):
-        y, xr, wr, aux, ctx.geom = _linear_forward(x, weight, bias, act, slope, residual, True)
+    def forward(ctx, x, weight, bias, residual, act, slope, device, code):
+        y, xr, wr, aux, ctx.geom = _linear_forward(x, weight, bias, act, slope, residual, device, code, True)
         ctx.save_for_backward(xr, wr, aux)
         return y
 
@@ -164,8 +169,8 @@ class _LinearFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         xr, wr, aux = ctx.saved_tensors
-        M, N, K, ldx, ldw, act, slope, code = ctx.geom
-        need_x, need_w, need_b, need_r, _, _ = ctx.needs_input_grad
+        M, N, K, ldx, ldw, act, slope, device, code = ctx.geom
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         like = torch.empty_like if M else torch.zeros_like
         dx = like(xr, memory_format=torch.contiguous_format) if need_x else None
         dw = like(wr, memory_format=torch.contiguous_format) if need_w else None
@@ -174,9 +179,9 @@ class _LinearFn(torch.autograd.Function):
             dyr, _, lddy = _rows(dy, N)
             lib = L.lib()
             ws = xr.new_empty(lib.vae_dense_workspace_floats(M, N, K, act, code), dtype=torch.float32)
-            _call(lib.vae_dense_backward, "vae_dense_backward", xr.device, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, wr.data_ptr(),
+            _call(lib.vae_dense_backward, "vae_dense_backward", device, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, wr.data_ptr(),
                   ldw, _p(aux), _p(dx), _p(dw), _p(db), ws.data_ptr(), M, N, K, act, slope, code)
-        return dx, dw, db, dy if need_r else None, None, None
+        return dx, dw, db, dy if need_r else None, None, None, None, None
 
 
 def linear(x, weight, bias=None, act="none", slope=0.0, residual=None):
@@ -185,23 +190,23 @@ def linear(x, weight, bias=None, act="none", slope=0.0, residual=None):
     x (..., K), weight (N, K), bias (N) or None, residual (..., N) or None, all of one type (fp32, bf16, fp16).  act: "none", "leaky"
     (negative side times `slope`; 0: ReLU), "sigmoid", "gelu" (the error function's), "silu".  One row runs as well as many:
     a served model's single tokens take a form of their own."""
-    L.require_device(x)
-    _dtype("linear", x)
+    device, code = _begin("linear", x)
     if act not in _ACTS:
         raise ValueError(f"linear: activation {act!r}, expected one of {', '.join(_ACTS)}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
-        raise ValueError(f"linear: input of shape {tuple(x.shape)} with a weight of shape {tuple(weight.shape)}")
+    shape = weight.shape
+    if len(shape) != 2 or x.dim() < 1 or x.shape[-1] != shape[1] or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"linear: input of shape {tuple(x.shape)} with a weight of shape {tuple(shape)}")
     kinds = (x.dtype,)
-    _same("linear", weight, "weight", weight.shape, kinds, x.device)
+    _same("linear", weight, "weight", shape, kinds, device)
     if bias is not None:
-        _same("linear", bias, "bias", weight.shape[:1], kinds, x.device)
+        _same("linear", bias, "bias", shape[:1], kinds, device)
         if not bias.is_contiguous():
             bias = bias.contiguous()
     if residual is not None:
-        _same("linear", residual, "residual", x.shape[:-1] + weight.shape[:1], kinds, x.device)
+        _same("linear", residual, "residual", x.shape[:-1] + shape[:1], kinds, device)
     if _needs_grad(x, weight, bias, residual):
-        return _LinearFn.apply(x, weight, bias, residual, _ACTS[act], float(slope))
-    return _linear_forward(x, weight, bias, _ACTS[act], float(slope), residual, False)[0]
+        return _LinearFn.apply(x, weight, bias, residual, _ACTS[act], float(slope), device, code)
+    return _linear_forward(x, weight, bias, _ACTS[act], float(slope), residual, device, code, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ gated scan
@@ -212,30 +217,30 @@ def _steps(t):
     return t, t.stride(0), t.stride(1)
 
 
-def _scan_forward(x, gate, h0, lengths, save):
+def _scan_forward(x, gate, h0, lengths, device, code, save):
     B, T, D = x.shape
-    dev = x.device
     xs, xb, xt = _steps(x)
     gs, gb, gt = _steps(gate)
     y = torch.empty_like(xs, memory_format=torch.contiguous_format)
     hl = xs.new_empty((B, D), dtype=torch.float32)
     kept = None
-    lib, code = L.lib(), _TYPES[x.dtype]
+    lib = L.lib()
     n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
     ws = xs.new_empty(n, dtype=torch.float32) if n else None
     if save:
         n = lib.vae_gated_scan_kept_floats(B, T, D)
         kept = xs.new_empty(n, dtype=torch.float32) if n else None
-    _call(lib.vae_gated_scan_forward, "vae_gated_scan_forward", dev, xs.data_ptr(), xb, xt, gs.data_ptr(), gb, gt, _p(h0),
+    _call(lib.vae_gated_scan_forward, "vae_gated_scan_forward", device, xs.data_ptr(), xb, xt, gs.data_ptr(), gb, gt, _p(h0),
           _p(lengths), y.data_ptr(), hl.data_ptr(), _p(kept), _p(ws), B, T, D, code)
     return y, hl, xs, gs, kept
 
 
 class _ScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, h0, lengths):
-        y, hl, xs, gs, kept = _scan_forward(x, gate, h0, lengths, True)
+    def forward(ctx, x, gate, h0, lengths, device, code):
+        y, hl, xs, gs, kept = _scan_forward(x, gate, h0, lengths, device, code, True)
         ctx.save_for_backward(xs, gs, h0, lengths, kept)
+        ctx.device, ctx.code = device, code
         ctx.set_materialize_grads(False)
         return y, hl
 
@@ -244,10 +249,9 @@ class _ScanFn(torch.autograd.Function):
     def backward(ctx, dy, dhl):
         xs, gs, h0, lengths, kept = ctx.saved_tensors
         B, T, D = xs.shape
-        dev = xs.device
-        need_x, need_g, need_h, _ = ctx.needs_input_grad
+        need_x, need_g, need_h = ctx.needs_input_grad[:3]
         if dy is None and dhl is None:
-            return None, None, None, None
+            return (None,) * 6
         dx = torch.empty_like(xs, memory_format=torch.contiguous_format) if need_x else None
         dg = torch.empty_like(xs, memory_format=torch.contiguous_format) if need_g else None
         dh0 = torch.empty_like(h0) if need_h else None
@@ -256,13 +260,13 @@ class _ScanFn(torch.autograd.Function):
             dy, db, dt = _steps(dy)
         if dhl is not None:
             dhl = dhl.contiguous()
-        lib, code = L.lib(), _TYPES[xs.dtype]
+        lib, code = L.lib(), ctx.code
         n = lib.vae_gated_scan_workspace_floats(B, T, D, code)
         ws = xs.new_empty(n, dtype=torch.float32) if n else None
-        _call(lib.vae_gated_scan_backward, "vae_gated_scan_backward", dev, _p(dy), db, dt, _p(dhl), xs.data_ptr(), xs.stride(0),
+        _call(lib.vae_gated_scan_backward, "vae_gated_scan_backward", ctx.device, _p(dy), db, dt, _p(dhl), xs.data_ptr(), xs.stride(0),
               xs.stride(1), gs.data_ptr(), gs.stride(0), gs.stride(1), _p(h0), _p(lengths), _p(kept), _p(dx), _p(dg), _p(dh0),
               _p(ws), B, T, D, code)
-        return dx, dg, dh0, None
+        return dx, dg, dh0, None, None, None
 
 
 def gated_scan(x, gate, h0=None, lengths=None):
@@ -272,23 +276,22 @@ def gated_scan(x, gate, h0=None, lengths=None):
     state before the first step (None: zeros); one step with h0 is how a served model advances.  lengths (B), int32 or int64 on
     the same device: steps at and behind a sequence's length are padding, whatever they hold; y is 0 there, the state stays.
     x and gate may be strided views with contiguous features (the halves of one projection)."""
-    L.require_device(x)
-    _dtype("gated_scan", x)
+    device, code = _begin("gated_scan", x)
     if x.dim() != 3:
         raise ValueError(f"gated_scan: input of shape {tuple(x.shape)}, expected (batch, steps, features)")
     B, T, D = x.shape
-    _same("gated_scan", gate, "gate", x.shape, (x.dtype,), x.device)
+    _same("gated_scan", gate, "gate", x.shape, (x.dtype,), device)
     if h0 is not None:
-        _same("gated_scan", h0, "h0", (B, D), (torch.float32,), x.device)
+        _same("gated_scan", h0, "h0", (B, D), (torch.float32,), device)
         if not h0.is_contiguous():
             h0 = h0.contiguous()
     if lengths is not None:
-        _same("gated_scan", lengths, "lengths", (B,), (torch.int32, torch.int64), x.device)
+        _same("gated_scan", lengths, "lengths", (B,), (torch.int32, torch.int64), device)
         if lengths.dtype != torch.int32 or not lengths.is_contiguous():
             lengths = lengths.clamp(0, T).to(torch.int32).contiguous()
     if B == 0 or T == 0 or D == 0:  # no step: the state stays
-        h = h0 if h0 is not None else torch.zeros(B, D, device=x.device)
+        h = h0 if h0 is not None else torch.zeros(B, D, device=device)
         return x * gate, h.clone()
     if _needs_grad(x, gate, h0):
-        return _ScanFn.apply(x, gate, h0, lengths)
-    return _scan_forward(x, gate, h0, lengths, False)[:2]
+        return _ScanFn.apply(x, gate, h0, lengths, device, code)
+    return _scan_forward(x, gate, h0, lengths, device, code, False)[:2]
