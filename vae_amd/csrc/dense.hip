@@ -234,7 +234,7 @@ __device__ __forceinline__ void aux_store8(void* aux, int64_t at, const float (&
 // columns, the same ones all the time, and a row leaves in whole lines: bias, what the backward pass needs, activation,
 // residual, store.  The residual is loaded two steps ahead.
 template <typename T, int FM, int FN>
-__device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)[FM][FN], int m0, int n0, int lane, float* sm) {
+__device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)[FM][FN], int m0, int n0, int slice, int lane, float* sm) {
     constexpr int LD = FN * 16 + 4, LPR = FN * 2, RPP = 64 / LPR, PASS = 32 / RPP;  // floats of a row in LDS, lanes a row, rows a pass
     const int n = n0 + lane % LPR * 8, left = g.N - n, r0 = lane / LPR;
     const float* mine = sm + r0 * LD + lane % LPR * 8;
@@ -273,7 +273,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
             if (has_res && row + 2 * RPP < end) load_raw<T, 8>(r2, res + (m + 2 * RPP) * g.ldr, left, g.N >= 8);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             if (plain) {
-                store_part<float, 8>(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, v, left);
+                store_part<float, 8>(g.part + ((int64_t)slice * g.M + m) * g.N + n, v, left);
                 continue;
             }
 #pragma unroll
@@ -289,12 +289,12 @@ __device__ __forceinline__ void store_tile(const GemmArgs& g, const f32x4 (&acc)
     }
 }
 
-// The tile of a workgroup.  Workgroups go round the 8 XCDs in turn, each with an L2 of its own: an XCD takes a contiguous share of
+// The `tile`-th tile.  Workgroups go round the 8 XCDs in turn, each with an L2 of its own: an XCD takes a contiguous share of
 // the tiles, in blocks 8 tiles of m high, so that its 32 CUs read 8 + 4 panels of the operands and not 32 + 32.
-__device__ __forceinline__ void tile_of(int M, int N, int BM, int BN, int& m, int& n) {
+__device__ __forceinline__ void tile_of(int tile, int M, int N, int BM, int BN, int& m, int& n) {
     const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, tiles = tm * tn;
-    const int x = blockIdx.x & 7, q = tiles >> 3, r = tiles & 7;
-    const int o = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
+    const int x = tile & 7, q = tiles >> 3, r = tiles & 7;
+    const int o = x * q + (x < r ? x : r) + (tile >> 3);
     const int per = 8 * tn, grp = o / per, in = o - grp * per;
     const int h = tm - grp * 8 < 8 ? tm - grp * 8 : 8;
     n = in / h;
@@ -306,15 +306,14 @@ __device__ __forceinline__ void tile_of(int M, int N, int BM, int BN, int& m, in
 // and only loads in flight hide that (64 x 4,096 x 4,096 bf16: TIMES).  The matrix instruction's first operand is B: a lane then
 // holds four neighbouring columns n of one row m of C.
 template <typename T, int BM, int BN, int WM, int WN, int AHEAD, bool ARC, bool BRC>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tile, int slice, char* lds) {
     constexpr int NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
-    extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int m0, n0;
-    tile_of(g.M, g.N, BM, BN, m0, n0);
+    tile_of(tile, g.M, g.N, BM, BN, m0, n0);
     m0 *= BM, n0 *= BN;
     const int wm = w % WM * (BM / WM), wn = w / WM * (BN / WN);
-    const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
+    const int k_lo = slice * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
     Stage<T, BM, ARC, NT> sa[AHEAD];
     Stage<T, BN, BRC, NT> sb[AHEAD];
     f32x4 acc[FM][FN];
@@ -359,7 +358,20 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_k(const GemmArgs g) {
             }
         }
     __syncthreads();
-    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
+    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, slice, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
+}
+template <typename T, int B, int AHEAD, bool ARC, bool BRC>
+__global__ __launch_bounds__(256) void gemm_k(const GemmArgs g) {
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    gemm_tile<T, B, B, 2, 2, AHEAD, ARC, BRC>(g, blockIdx.x, blockIdx.z, lds);
+}
+// dW and dx of a small layer side by side: neither fills the chip, and a launch is saved.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_pair_k(const GemmArgs dw, int dw_tiles, int dw_blocks, const GemmArgs dx) {
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    const int i = blockIdx.x;
+    if (i < dw_blocks) gemm_tile<T, 64, 64, 2, 2, 4, true, true>(dw, i % dw_tiles, i / dw_tiles, lds);
+    else gemm_tile<T, 64, 64, 2, 2, 4, false, true>(dx, i - dw_blocks, 0, lds);
 }
 
 // ---- The large products -----------------------------------------------------------------------------------------------
@@ -433,7 +445,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
     extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int m0, n0;
-    tile_of(g.M, g.N, BM, BN, m0, n0);
+    tile_of(blockIdx.x, g.M, g.N, BM, BN, m0, n0);
     m0 *= BM, n0 *= BN;
     const int wm = (w & 1) * (BM / 2), wn = (w >> 1) * (BN / 2);
     const int k_lo = blockIdx.z * g.kslice, k_hi = g.K - k_lo < g.kslice ? g.K : k_lo + g.kslice;
@@ -505,7 +517,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
     static_assert(2 * DN <= FM && RPR <= FN, "a phase holds the loads and the reads");
     // (the loads behind the last tile bring nothing, but they must have ended before LDS is used for something else)
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
+    store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, blockIdx.z, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
 
 // ---- Few rows (serving) --------------------------------------------------------------------------------------------------
@@ -582,19 +594,34 @@ int dense_rows(const GemmArgs& g, hipStream_t s) {
     return VAE_OK;
 }
 
-// c = sum of the slices of a split product, in a fixed order
+// What the backward pass leaves in parts, added in a fixed order: the first join_blocks workgroups add the slices of dW (1024 values
+// each), the others the rows of db's partial sums (64 columns each, four waves that take every fourth row).
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_join_k(const float* part, int slices, int64_t n, T* c) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    float s[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
+__global__ __launch_bounds__(256) void dense_join_k(const float* part, int slices, int64_t n, T* c, int join_blocks, const float* cols, int rows,
+                                                    int N, T* db) {
+    if ((int)blockIdx.x < join_blocks) {
+        const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+        if (i >= n) return;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
 #pragma unroll 4
-    for (int k = 0; k < slices; ++k) {
-        load_part<float, 4>(v, part + k * n + i, n - i);
+        for (int k = 0; k < slices; ++k) {
+            load_part<float, 4>(v, part + k * n + i, n - i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
+            for (int e = 0; e < 4; ++e) s[e] += v[e];
+        }
+        store_part<T, 4>(c + i, s, n - i);
+        return;
     }
-    store_part<T, 4>(c + i, s, n - i);
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = ((int)blockIdx.x - join_blocks) * 64 + lane;
+    float s = 0.f;
+    if (col < N) {
+#pragma unroll 8
+        for (int r = w; r < rows; r += 4) s += cols[(int64_t)r * N + col];
+    }
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && col < N) db[col] = (T)(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
 }
 
 // dp = dy act'(p), rounded to the type of the products that read it (the matrix cores take their operands so), and the column sums
@@ -647,13 +674,13 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
     part[(int64_t)blockIdx.y * N + at] = t;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ARC, bool BRC, bool DMA>
+template <typename T, int BM, int BN, bool ARC, bool BRC, bool DMA>
 int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     constexpr int bytes = 2 * (BM + BN) * KB;
-    static_assert(WM * WN * 32 * (BN / WN + 4) * 4 <= bytes, "the epilogue's LDS");
+    static_assert(4 * 32 * (BN / 2 + 4) * 4 <= bytes && BM == BN, "the epilogue's LDS");
     void (*k)(const GemmArgs);
     if constexpr (DMA) k = gemm_dma_k<T, BM, BN, ARC, BRC>;
-    else k = gemm_k<T, BM, BN, WM, WN, BM == 64 ? 4 : 2, ARC, BRC>;
+    else k = gemm_k<T, BM, BM == 64 ? 4 : 2, ARC, BRC>;
     if (bytes > 65536) {
         static uint64_t granted = 0;  // per device; a race only repeats the call
         int dev = 0;
@@ -665,7 +692,7 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     }
     const int64_t tiles = ceil_div64(g.N, BN) * ceil_div64(g.M, BM);
     if (tiles > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "gemm: %lld tiles", (long long)tiles);
-    k<<<dim3((unsigned)tiles, 1, slices), dim3(WM * WN * 64), bytes, s>>>(g);
+    k<<<dim3((unsigned)tiles, 1, slices), dim3(256), bytes, s>>>(g);
     VAE_LAUNCH_CHECK("gemm_k");
     return VAE_OK;
 }
@@ -697,29 +724,15 @@ int gemm_slices(int64_t M, int64_t N, int64_t K, int bk, int* kslice) {
     return (int)ceil_div64(kt, per);
 }
 
+// slices > 1: g.part holds the sums, the caller adds them up
 template <typename T, bool ARC, bool BRC>
-int gemm(GemmArgs g, float* part, hipStream_t s) {
-    int slices = 1;
-    g.part = nullptr;
-    g.kslice = g.K;
-    if (part != nullptr) {
-        slices = gemm_slices(g.M, g.N, g.K, BK<T>(), &g.kslice);
-        if (slices > 1) g.part = part;
+int gemm(const GemmArgs& g, int slices, hipStream_t s) {
+    if (gemm_small(g.M, g.N)) return gemm_inst<T, 64, 64, ARC, BRC, false>(g, slices, s);
+    if (!whole_pieces<T>(g, ARC, BRC)) return gemm_inst<T, 128, 128, ARC, BRC, false>(g, slices, s);
+    if constexpr (sizeof(T) == 2) {
+        if (gemm_large(g.M, g.N)) return gemm_inst<T, 256, 256, ARC, BRC, true>(g, slices, s);
     }
-    int rc;
-    if (gemm_small(g.M, g.N)) rc = gemm_inst<T, 64, 64, 2, 2, ARC, BRC, false>(g, slices, s);
-    else if (whole_pieces<T>(g, ARC, BRC)) {
-        rc = VAE_EINVAL;
-        if constexpr (sizeof(T) == 2) {
-            if (gemm_large(g.M, g.N)) rc = gemm_inst<T, 256, 256, 2, 2, ARC, BRC, true>(g, slices, s);
-            else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, true>(g, slices, s);
-        } else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, true>(g, slices, s);
-    } else rc = gemm_inst<T, 128, 128, 2, 2, ARC, BRC, false>(g, slices, s);
-    if (rc != VAE_OK || slices == 1) return rc;
-    const int64_t n = (int64_t)g.M * g.N;
-    gemm_join_k<T><<<dim3((unsigned)ceil_div64(n, 1024)), dim3(256), 0, s>>>(part, slices, n, (T*)g.c);
-    VAE_LAUNCH_CHECK("gemm_join_k");
-    return VAE_OK;
+    return gemm_inst<T, 128, 128, ARC, BRC, true>(g, slices, s);
 }
 
 // Slices of the rows: about 2048 workgroups in all, 256 at most (rows of partial sums)
@@ -754,30 +767,35 @@ template <typename T>
 int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, int64_t ldw, const void* aux, T* dx, T* dw, T* db, float* ws,
                      int M, int N, int K, int act, float slope, int dtype, hipStream_t s) {
     const DenseWs lay = dense_ws(M, N, K, dtype, act);
-    const int auxk = aux_kind(act, dtype);
+    const int auxk = aux_kind(act, dtype), ny = dact_rows(M, N);
     const T* dp = dy;
     int64_t lddp = lddy;
     if (auxk != AUX_NONE || db != nullptr) {
         T* out = (T*)(ws + lay.dp);
-        const int ny = dact_rows(M, N);
-        float* cols = db != nullptr ? ws + lay.cols : nullptr;
-        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, dp_stride(N, sizeof(T)), cols, M, N, act, auxk, slope);
+        dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, dp_stride(N, sizeof(T)),
+                                                                                   db != nullptr ? ws + lay.cols : nullptr, M, N, act, auxk, slope);
         VAE_LAUNCH_CHECK("dense_dact_k");
         if (auxk != AUX_NONE) dp = out, lddp = dp_stride(N, sizeof(T));
-        if (db != nullptr) {
-            part_cols_k<T><<<dim3((unsigned)ceil_div64(N, 64)), dim3(1024), 0, s>>>(cols, ny, N, db, nullptr, N);
-            VAE_LAUNCH_CHECK("part_cols_k");
-        }
     }
-    if (dx != nullptr) {
-        GemmArgs g = {};
-        g.a = dp, g.lda = lddp, g.b = w, g.ldb = ldw, g.c = dx, g.ldc = K, g.M = M, g.N = K, g.K = N;
-        if (int rc = gemm<T, false, true>(g, nullptr, s)) return rc;
+    GemmArgs gx = {}, gw = {};
+    gx.a = dp, gx.lda = lddp, gx.b = w, gx.ldb = ldw, gx.c = dx, gx.ldc = K, gx.M = M, gx.N = K, gx.K = N, gx.kslice = N;
+    gw.a = dp, gw.lda = lddp, gw.b = x, gw.ldb = ldx, gw.c = dw, gw.ldc = K, gw.M = N, gw.N = K, gw.K = M;
+    const int slices = gemm_slices(N, K, M, BK<T>(), &gw.kslice);
+    if (slices > 1) gw.part = ws + lay.split;
+    const int64_t tx = ceil_div64(M, 64) * ceil_div64(K, 64), tw = ceil_div64(N, 64) * ceil_div64(K, 64);
+    if (dx != nullptr && dw != nullptr && gemm_small(M, K) && gemm_small(N, K)) {
+        gemm_pair_k<T><<<dim3((unsigned)(tw * slices + tx)), dim3(256), 2 * 128 * KB, s>>>(gw, (int)tw, (int)(tw * slices), gx);
+        VAE_LAUNCH_CHECK("gemm_pair_k");
+    } else {
+        if (dx != nullptr)
+            if (int rc = gemm<T, false, true>(gx, 1, s)) return rc;
+        if (dw != nullptr)
+            if (int rc = gemm<T, true, true>(gw, slices, s)) return rc;
     }
-    if (dw != nullptr) {
-        GemmArgs g = {};
-        g.a = dp, g.lda = lddp, g.b = x, g.ldb = ldx, g.c = dw, g.ldc = K, g.M = N, g.N = K, g.K = M;
-        if (int rc = gemm<T, true, true>(g, ws + lay.split, s)) return rc;
+    const int64_t n = (int64_t)N * K, join = dw != nullptr && slices > 1 ? ceil_div64(n, 1024) : 0, sums = db != nullptr ? ceil_div64(N, 64) : 0;
+    if (join + sums > 0) {
+        dense_join_k<T><<<dim3((unsigned)(join + sums)), dim3(256), 0, s>>>(ws + lay.split, slices, n, dw, (int)join, ws + lay.cols, ny, N, db);
+        VAE_LAUNCH_CHECK("dense_join_k");
     }
     return VAE_OK;
 }
@@ -807,10 +825,11 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.c = y, g.ldc = ldy, g.bias = bias, g.res = res, g.ldr = ldr;
     g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
     g.aux = g.auxk == AUX_NONE ? nullptr : aux;
+    g.kslice = K;
     hipStream_t s = (hipStream_t)stream;
     if (M <= ROWS_MAX) return dtype == VAE_T_F32 ? dense_rows<float>(g, s) : dtype == VAE_T_BF16 ? dense_rows<bf16_t>(g, s) : dense_rows<f16_t>(g, s);
-    if (dtype == VAE_T_F32) return gemm<float, false, false>(g, nullptr, s);
-    return dtype == VAE_T_BF16 ? gemm<bf16_t, false, false>(g, nullptr, s) : gemm<f16_t, false, false>(g, nullptr, s);
+    if (dtype == VAE_T_F32) return gemm<float, false, false>(g, 1, s);
+    return dtype == VAE_T_BF16 ? gemm<bf16_t, false, false>(g, 1, s) : gemm<f16_t, false, false>(g, 1, s);
 }
 
 extern "C" int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype) {
