@@ -47,13 +47,13 @@ struct GsLane {
 };
 template <int V>
 __device__ __forceinline__ GsLane gs_lane(const GsArgs& a) {
-    const int dv = (a.D + V - 1) / V;
-    int64_t q = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const uint32_t dv = ((uint32_t)a.D + V - 1) / V, n = a.B * dv;  // (n <= B D < 2^31)
+    uint32_t q = blockIdx.x * 64 + (threadIdx.x & 63);
     GsLane l;
-    l.stores = q < (int64_t)a.B * dv;
-    if (!l.stores) q = (int64_t)a.B * dv - 1;
+    l.stores = q < n;
+    if (!l.stores) q = n - 1;
     l.b = (int)(q / dv);
-    l.d = (int)(q - (int64_t)l.b * dv) * V;
+    l.d = (int)(q - l.b * dv) * V;
     if (l.d > a.D - V) l.d = a.D - V;
     l.len = a.lengths != nullptr ? a.lengths[l.b] : a.T;
     l.len = l.len > a.T ? a.T : l.len < 0 ? 0 : l.len;
