@@ -6,6 +6,8 @@
 // One product kernel serves all three: C[m][n] = sum_k A(m, k) B(n, k), each operand stored either with k contiguous (x and W in
 // the forward pass, dp in dx) or with its row contiguous (W in dx; dp and x in dW).  Products run on the matrix cores, sums in
 // fp32.
+#include <atomic>
+
 #include "seqops.h"
 
 namespace {
@@ -682,12 +684,12 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     if constexpr (DMA) k = gemm_dma_k<T, BM, BN, ARC, BRC>;
     else k = gemm_k<T, BM, BM == 64 ? 4 : 2, ARC, BRC>;
     if (bytes > 65536) {
-        static uint64_t granted = 0;  // per device; a race only repeats the call
+        static std::atomic<uint64_t> granted{0};  // a bit a device (two threads at once both ask, which does no harm)
         int dev = 0;
         VAE_HIP(hipGetDevice(&dev));
-        if (dev < 64 && !(granted >> dev & 1)) {
+        if (dev >= 64 || !(granted.load(std::memory_order_relaxed) >> dev & 1)) {
             VAE_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-            granted |= (uint64_t)1 << dev;
+            if (dev < 64) granted.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
         }
     }
     const int64_t tiles = ceil_div64(g.N, BN) * ceil_div64(g.M, BM);

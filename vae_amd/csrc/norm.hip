@@ -8,6 +8,8 @@
 // alone; longer rows take a workgroup.  The backward pass keeps dw and db of the lane's own columns in registers over all rows
 // that its group visits; workgroups leave one row of partials each, which a second launch adds in a fixed order (no atomics:
 // two runs give the same bits).
+#include <atomic>
+
 #include "seqops.h"
 
 namespace {
@@ -385,11 +387,13 @@ template <typename T, typename TW, int G, int NCH>
 int bwd_inst(const NormArgs& a) {
     constexpr int NT = norm_threads<G>();
     const bool cols = a.dw != nullptr || a.db != nullptr;
-    static int resident = 0;  // workgroups that the chip holds at once (the same on every device; a race only repeats the query)
+    static std::atomic<int> known{0};  // workgroups that the chip holds at once, the same on every device
+    int resident = known.load(std::memory_order_relaxed);
     if (resident == 0) {
         int cu = 0;
         VAE_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&cu, norm_bwd_k<T, TW, G, NCH>, NT, 0));
         resident = 256 * (cu < 1 ? 1 : cu);
+        known.store(resident, std::memory_order_relaxed);
     }
     int64_t n = ceil_div64(a.rows, NT / G);
     if (n > norm_parts_cap(a.C)) n = norm_parts_cap(a.C);

@@ -7,7 +7,6 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
 static inline int vae_type_size(int t) { return t == VAE_T_F32 ? 4 : (t == VAE_T_BF16 || t == VAE_T_F16) ? 2 : 0; }
-static inline const char* vae_type_name(int t) { return t == VAE_T_F32 ? "f32" : t == VAE_T_BF16 ? "bf16" : t == VAE_T_F16 ? "f16" : "?"; }
 
 // N elements that start on any multiple of the element's size: gfx950's global loads and stores take such addresses, so
 // rows of odd length move in 16-byte pieces like aligned ones.
