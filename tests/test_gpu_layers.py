@@ -332,6 +332,22 @@ def test_linear_far_values_and_nan_rows():
         assert torch.equal(y[keep], clean[keep])
 
 
+def test_linear_one_row_of_any_stride():
+    """Through the C entry: the strides of a single row say nothing, 0 among them.  Products of two bf16 values are exact in fp32, so
+    dW is its own rounding; dx: a sum of n terms."""
+    from vae_amd import _lib as L
+    n = k = 2048
+    x, dy, w = (rnd(s, torch.bfloat16, 70 + i) for i, s in enumerate(((1, k), (1, n), (n, k))))
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    lib = L.lib()
+    ws = torch.empty(lib.vae_dense_workspace_floats(1, n, k, L.ACT_NONE, L.T_BF16), device="cuda")
+    L.check(lib.vae_dense_backward(dy.data_ptr(), 0, x.data_ptr(), 0, w.data_ptr(), k, None, dx.data_ptr(), dw.data_ptr(), None,
+                                   ws.data_ptr(), 1, n, k, L.ACT_NONE, 0.0, L.T_BF16, L.stream_ptr()), "vae_dense_backward")
+    assert torch.equal(dw, (dy.float().t() * x.float()).bfloat16())
+    terms = dy.double().t() * w.double()
+    check("dx", dx, terms.sum(0, keepdim=True), n * U * terms.abs().sum(0, keepdim=True))
+
+
 def test_linear_only_the_gradients_asked_for():
     from vae_amd import layers
     x, w, b, dy = rnd((40, 96), torch.float32, 1), rnd((32, 96), torch.float32, 2), rnd((32,), torch.float32, 3), rnd((40, 32), torch.float32, 5)

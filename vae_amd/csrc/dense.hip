@@ -823,6 +823,7 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
     if (M == 0) return VAE_OK;
     if (x == nullptr || w == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null buffer");
     if ((M > 1 && (ldx < K || ldy < N || (res != nullptr && ldr < N))) || (N > 1 && ldw < K)) VAE_FAIL(VAE_EINVAL, "dense_forward: a row stride below the row");
+    if (N == 1) ldw = K;  // (a single row's stride may be anything)
     GemmArgs g = {};
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.c = y, g.ldc = ldy, g.bias = bias, g.res = res, g.ldr = ldr;
     g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
@@ -847,6 +848,8 @@ extern "C" int vae_dense_backward(const void* dy, int64_t lddy, const void* x, i
     if (dy == nullptr || x == nullptr || w == nullptr || workspace == nullptr || (act != VAE_ACT_NONE && aux == nullptr))
         VAE_FAIL(VAE_EINVAL, "dense_backward: null buffer");
     if ((M > 1 && (ldx < K || lddy < N)) || (N > 1 && ldw < K)) VAE_FAIL(VAE_EINVAL, "dense_backward: a row stride below the row");
+    if (M == 1) ldx = K, lddy = N;  // (a single row's stride may be anything)
+    if (N == 1) ldw = K;
     hipStream_t s = (hipStream_t)stream;
 #define VAE_DENSE(T) \
     return dense_backward_t<T>((const T*)dy, lddy, (const T*)x, ldx, (const T*)w, ldw, aux, (T*)dx, (T*)dw, (T*)db, workspace, M, N, K, act, slope, dtype, s)
