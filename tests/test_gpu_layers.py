@@ -475,6 +475,14 @@ def test_scan_long_with_few_channels(dtype):
     scan_compare(run_scan(x, gate, h0, lengths, dy, dhl), scan64(x, gate, h0, lengths, dy, dhl))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("b, t, d", [(8, 600, 600), (9, 530, 1001)])
+def test_scan_between_few_and_many_channels(b, t, d, dtype):
+    """Channels for which the two passes cut the time axis differently."""
+    x, gate, h0, dy, dhl = scan_inputs(b, t, d, dtype)
+    scan_compare(run_scan(x, gate, h0, None, dy, dhl), scan64(x, gate, h0, None, dy, dhl))
+
+
 def test_scan_strided_views():
     from vae_amd import layers
     for dtype in DTYPES:

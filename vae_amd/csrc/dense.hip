@@ -3,9 +3,12 @@
 //   p = x W^T + b,  y = act(p) + r        x: M x K, W: N x K (row-major), y, r: M x N
 //   dp = dy act'(p),  dx = dp W,  dW = dp^T x,  db = sum over rows of dp,  dr = dy
 //
-// One product kernel serves all three: C[m][n] = sum_k A(m, k) B(n, k), each operand stored either with k contiguous (x and W in
-// the forward pass, dp in dx) or with its row contiguous (W in dx; dp and x in dW).  Products run on the matrix cores, sums in
-// fp32.
+// All three are C[m][n] = sum_k A(m, k) B(n, k), each operand stored either with k contiguous (x and W in the forward pass, dp in
+// dx) or with its row contiguous (W in dx; dp and x in dW).  Products run on the matrix cores, sums in fp32, in one of four
+// kernels: dense_rows_k (forward, up to 64 rows: bound by the weight's bytes), gemm_k (operands of any alignment and products too
+// small for 128 x 128 tiles: bound by latency), gemm_dma_k (the others: bound by the matrix cores and the clock that their power
+// leaves them), gemm_pair_k (dW and dx of a small layer in one launch).  Around the products of a backward pass stand a pass that makes
+// dp and its column sums (dense_dact_k: bytes) and one that adds the slices of dW and the partial sums of db (dense_join_k).
 #include <atomic>
 
 #include "seqops.h"
@@ -305,7 +308,7 @@ __device__ __forceinline__ void tile_of(int tile, int M, int N, int BM, int BN, 
 
 // C tile BM x BN by WM x WN waves, for products too small for the kernel below and for operands of any alignment.  The tiles of
 // the operands pass registers, AHEAD of them in flight: with a workgroup or two a CU a tile's loads take longer than its products,
-// and only loads in flight hide that (64 x 4,096 x 4,096 bf16: TIMES).  The matrix instruction's first operand is B: a lane then
+// and only loads in flight hide that (256 x 4,096 x 4,096 bf16 forward: 46 us with one tile ahead, 29 with four).  The matrix instruction's first operand is B: a lane then
 // holds four neighbouring columns n of one row m of C.
 template <typename T, int BM, int BN, int WM, int WN, int AHEAD, bool ARC, bool BRC>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tile, int slice, char* lds) {
@@ -435,11 +438,17 @@ struct Dma {
 };
 
 // One wave a SIMD with a 128 x 128 (BM = BN = 256) share of C in its accumulators: a fragment read from LDS then serves eight matrix
-// instructions, and LDS moves 96 bytes a cycle (with 64 x 128 shares it would be 128, all that it can).  (BM = BN = 128: two workgroups
-// a CU, for products with too few tiles of 256.)  The k-loop runs in phases of 64 bytes of k.  In phase h the matrix cores work on the fragments of half tile h, the fragments of h + 1 are read, and the loads
-// of h + 4 are issued into the slot of a ring of four that h has left: a load has two phases and more to arrive.  One barrier a phase
-// says that h + 2 has landed for every wave and that h + 1 has been read by every wave.  Reads and loads stand between the matrix
-// instructions, one at a time, where their issue costs nothing.
+// instructions, and LDS moves 96 bytes a cycle (with 64 x 128 shares it would be 128, all that it can).  BM = BN = 128: two
+// workgroups a CU, for products with too few tiles of 256, and for fp32, where 256 does not leave the fragments registers enough.
+//   The k-loop runs in phases of 64 bytes of k.  In phase h the matrix cores work on the fragments of half tile h, the fragments of
+// h + 1 are read, and the loads of h + 4 are issued into the slot of a ring of four that h has left: a load has two phases and more
+// to arrive.  One barrier a phase says that h + 2 has landed for every wave and that h + 1 has been read by every wave.  Reads and
+// loads stand between the matrix instructions, one at a time, where their issue costs nothing.
+//   16,384 x 4,096 x 4,096 bf16 (0.55 TFLOP each): forward with bias, GELU, residual and what its derivative needs 614 us, dx 465
+// (1.18 PFLOP/s), dW 403 (1.36); register-staged 128 x 128 tiles: 938, 736, 662.
+// The clock falls to 1.5 to 1.9 GHz meanwhile, so what saves waits alone gains nothing: workgroups that stay and load into their
+// next tile during the epilogue measured 634 us forward, whole 128-byte lines of k 418 against 449 for a bare forward product but
+// registers beyond the file for dW, 32 x 32 matrix instructions 855 against 849.
 template <typename T, int BM, int BN, bool ARC, bool BRC>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmArgs g) {
     constexpr int NT = 256, V = 16 / sizeof(T), FM = BM / 32, FN = BN / 32, SLOT = (BM + BN) * HB;
@@ -525,7 +534,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
 // ---- Few rows (serving) --------------------------------------------------------------------------------------------------
 // y of up to 64 rows: the weight's bytes are the bound, so they are read once and straight into registers.  A workgroup takes 16
 // columns of y (rows of w) and shares k out among its waves; each wave has eight 1-KiB loads in flight, multiplies them on the matrix
-// cores with MF x 16 rows of x (zeros where there are fewer), and the waves' sums meet in LDS.
+// cores with MF x 16 rows of x (zeros where there are fewer), and the waves' sums meet in LDS.  4,096 x 4,096 bf16, one row: 11 us a
+// call (a third of it launch; 33.6 MB would take 6.6).  Up to 64 rows, as the tiles of gemm_k are 64 high: less would be padding there.
 constexpr int ROWS_MAX = 64, ROWS_STEPS = 8;
 template <typename T, int MF>
 __global__ __launch_bounds__(MF == 4 ? 512 : 1024) void dense_rows_k(const GemmArgs g, int steps) {  // steps: pieces of 64 bytes of k a wave takes

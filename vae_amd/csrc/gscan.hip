@@ -429,7 +429,11 @@ int64_t gs_columns(int B, int D, int V) { return ceil_div64((int64_t)B * ((D + V
 
 // What a launch looks like: V features a lane (as many as leave 256 columns of workgroups; at most 8 bytes forward, 8 and 4 bytes
 // (fp32 and 16-bit types) backward, where more would not stay in registers; never more than D), W waves a workgroup, parts of the
-// time axis.
+// time axis, as many as make 512 workgroups.  Parts read x and gate (backward: gate and dy) twice, but let more workgroups at them than
+// the channels make.  In parts and in one go, T = 4,096: fp32 forward 31 and 62 us at 24 columns, 60 and 62 at 64, 70 and 63 at 72 (T =
+// 16,384: 266 and 307 at 64, 331 and 333 at 80), backward 161 and 164 at 104, 191 and 181 at 128; bf16 forward 43 and 61 at 64, 53 and
+// 61 at 80, 63 and 61 at 88, backward 106 and 137 at 128, 137 and 131 at 144.  Below four tiles there is little to share out (T = 512
+// forward: 14 and 10).
 struct GsPlan {
     int V, W, parts, part_steps;
 };
@@ -440,7 +444,8 @@ GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
     const int64_t cols = gs_columns(B, D, p.V);
     p.W = T <= GS_S ? 1 : T <= 4 * GS_S ? 4 : cols >= 512 || T <= GS_TILE || p.V > 1 ? 8 : 16;
     const int64_t tile = p.W * (fwd ? gs_steps(p.W) : GS_S), tiles = ceil_div64(T, tile);
-    int64_t n = cols >= 192 ? 1 : ceil_div64(512, cols);
+    const int64_t enough = fwd ? (esize == 4 ? 72 : 88) : (esize == 4 ? 112 : 136);
+    int64_t n = cols >= enough || tiles < 4 ? 1 : 512 / cols;
     if (n > GS_MAX_PARTS) n = GS_MAX_PARTS;
     if (n > tiles) n = tiles;
     const int64_t per = ceil_div64(tiles, n);
@@ -452,7 +457,7 @@ GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
 template <typename T, int V, int W, bool FWD>
 int gs_launch(const GsArgs& a) {
     const dim3 grid((unsigned)gs_columns(a.B, a.D, V), a.parts);
-    if constexpr (W >= 8) {
+    if constexpr (W == 16) {  // (fewer waves: a short series, or channels enough)
         if (a.parts > 1) {
             if (FWD) gscan_fwd_k<T, V, W, gs_steps(W), true><<<grid, dim3(W * 64), 0, a.s>>>(a);
             else gscan_bwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
