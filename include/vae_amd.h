@@ -342,12 +342,15 @@ int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
                             int dtype, int wtype, vae_stream_t stream);
 
 /* Linear layer p = x w^T + bias, y = act(p) + res: x M x K, w N x K, res and y M x N; bias (N), res optional.  act = VAE_ACT_*
- * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.
+ * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.  workspace
+ * (vae_dense_forward_workspace_floats; NULL where that is 0): sums of products of few outputs, which are split over k.
  * Backward: dp = dy act'(p); dx = dp w (M x K, dense), dw = dp^T x (N x K, dense), db = column sums of dp; each optional.  The
  * residual's gradient is dy itself. */
 int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype);
 int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
-                      void* y, int64_t ldy, void* aux, int M, int N, int K, int act, float slope, int dtype, vae_stream_t stream);
+                      void* y, int64_t ldy, void* aux, float* workspace, int M, int N, int K, int act, float slope, int dtype,
+                      vae_stream_t stream);
+int64_t vae_dense_forward_workspace_floats(int64_t M, int64_t N, int64_t K, int dtype);
 int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype);
 int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* aux,
                        void* dx, void* dw, void* db, float* workspace, int M, int N, int K, int act, float slope, int dtype,

@@ -281,6 +281,22 @@ def test_linear_large_tiles(m, n, k, dtype):
     linear_case(m, n, k, dtype, "none", bias=True, residual=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(4100, 2568, 264), (4100, 264, 2568), (264, 4104, 2568)])
+def test_linear_largest_tiles(m, n, k, dtype):
+    """Forward, dx and dW in turn are the product of many outputs."""
+    linear_case(m, n, k, dtype, "silu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(100, 70, 4000), (65, 1, 2001), (100, 4000, 70), (70, 4000, 4001), (300, 500, 8000), (2000, 1030, 2048)])
+@pytest.mark.parametrize("act", ["leaky", "gelu"])
+def test_linear_few_outputs_of_long_sums(m, n, k, dtype, act):
+    """Sums of thousands of terms for few outputs: split over k."""
+    linear_case(m, n, k, dtype, act)
+    linear_case(m, n, k, dtype, "none", bias=False, residual=False)
+
+
 def test_linear_strides():
     from vae_amd import layers
     for dtype in DTYPES:

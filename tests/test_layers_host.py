@@ -37,16 +37,19 @@ def test_layer_norm_entry_checks():
 def test_dense_entry_checks():
     from vae_amd import _lib as L
     lib, p = L.lib(), 4096
-    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, 2, 4, 8, 0, 0.0, 9, None), "type")
-    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, 2, 4, 8, 5, 0.0, 0, None), "activation")
-    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, 2, 0, 8, 0, 0.0, 0, None), "N = 0")
-    _fails(lib.vae_dense_forward(p, 8, None, 8, None, None, 0, p, 4, None, 2, 4, 8, 0, 0.0, 0, None), "null")
-    _fails(lib.vae_dense_forward(p, 7, p, 8, None, None, 0, p, 4, None, 2, 4, 8, 0, 0.0, 0, None), "stride")
-    _fails(lib.vae_dense_forward(p, 8, p, 8, None, p, 3, p, 4, None, 2, 4, 8, 0, 0.0, 0, None), "stride")
+    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, None, 2, 4, 8, 0, 0.0, 9, None), "type")
+    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, None, 2, 4, 8, 5, 0.0, 0, None), "activation")
+    _fails(lib.vae_dense_forward(p, 8, p, 8, None, None, 0, p, 4, None, None, 2, 0, 8, 0, 0.0, 0, None), "N = 0")
+    _fails(lib.vae_dense_forward(p, 8, None, 8, None, None, 0, p, 4, None, None, 2, 4, 8, 0, 0.0, 0, None), "null")
+    _fails(lib.vae_dense_forward(p, 7, p, 8, None, None, 0, p, 4, None, None, 2, 4, 8, 0, 0.0, 0, None), "stride")
+    _fails(lib.vae_dense_forward(p, 8, p, 8, None, p, 3, p, 4, None, None, 2, 4, 8, 0, 0.0, 0, None), "stride")
+    assert lib.vae_dense_forward_workspace_floats(100, 8, 4096, L.T_F32) >= 2 * 100 * 8  # few outputs, a long sum: split
+    _fails(lib.vae_dense_forward(p, 4096, p, 4096, None, None, 0, p, 8, None, None, 100, 8, 4096, 0, 0.0, 0, None), "workspace")
+    assert [lib.vae_dense_forward_workspace_floats(*a) for a in ((1, 8, 4096, 0), (100, 8, 64, 0), (4096, 4096, 4096, 0), (0, 8, 64, 0))] == [0] * 4
     _fails(lib.vae_dense_backward(p, 4, p, 8, p, 8, None, p, p, p, p, 2, 4, 8, L.ACT_GELU, 0.0, 0, None), "null")
     _fails(lib.vae_dense_backward(p, 4, p, 8, p, 8, None, p, p, p, None, 2, 4, 8, 0, 0.0, 0, None), "null")
     _fails(lib.vae_dense_backward(p, 4, p, 8, p, 8, None, p, p, p, p, 0, 4, 8, 0, 0.0, 0, None), "no rows")
-    assert lib.vae_dense_forward(None, 8, None, 8, None, None, 0, None, 4, None, 0, 4, 8, 0, 0.0, 0, None) == 0
+    assert lib.vae_dense_forward(None, 8, None, 8, None, None, 0, None, 4, None, None, 0, 4, 8, 0, 0.0, 0, None) == 0
     # what act' needs: a byte for the leaky ReLU, fp16 behind bf16 tensors, fp32 else
     assert [lib.vae_dense_aux_bytes(3, 5, a, L.T_BF16) for a in range(5)] == [0, 15, 30, 30, 30]
     assert [lib.vae_dense_aux_bytes(3, 5, a, L.T_F16) for a in range(5)] == [0, 15, 60, 60, 60]

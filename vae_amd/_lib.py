@@ -102,15 +102,16 @@ def lib():
     L.vae_layer_norm_workspace_floats.argtypes = [i64, i32]
     L.vae_layer_norm_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
     L.vae_dense_aux_bytes.argtypes = [i64, i64, i32, i32]
-    L.vae_dense_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i32, i32, i32, i32, f32, i32, vp]
+    L.vae_dense_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, f32, i32, vp]
+    L.vae_dense_forward_workspace_floats.argtypes = [i64, i64, i64, i32]
     L.vae_dense_workspace_floats.argtypes = [i64, i64, i64, i32, i32]
     L.vae_dense_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]
     L.vae_gated_scan_kept_floats.argtypes = [i32, i32, i32]
     L.vae_gated_scan_workspace_floats.argtypes = [i32, i32, i32, i32]
     L.vae_gated_scan_forward.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
     L.vae_gated_scan_backward.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
-    for name in ("vae_layer_norm_workspace_floats", "vae_dense_aux_bytes", "vae_dense_workspace_floats", "vae_gated_scan_kept_floats",
-                 "vae_gated_scan_workspace_floats"):
+    for name in ("vae_layer_norm_workspace_floats", "vae_dense_aux_bytes", "vae_dense_forward_workspace_floats",
+                 "vae_dense_workspace_floats", "vae_gated_scan_kept_floats", "vae_gated_scan_workspace_floats"):
         getattr(L, name).restype = i64
     L.vae_graph_begin.argtypes = [ctypes.POINTER(vp)]
     L.vae_graph_end.argtypes = [ctypes.POINTER(vp)]
@@ -135,7 +136,7 @@ EXPORTS = ("vae_seq_scratch_floats", "vae_last_error", "vae_check_device", "vae_
            "vae_graph_launch", "vae_graph_destroy", "vae_dp_unique_id", "vae_dp_init", "vae_dp_world", "vae_dp_enable",
            "vae_dp_all_gather_rows", "vae_dp_all_reduce_sum", "vae_dp_shutdown", "vae_run_backward_step",
            "vae_dp_set_single_comm", "vae_dp_single_comm", "vae_time_step", "vae_layer_norm_forward", "vae_layer_norm_workspace_floats",
-           "vae_layer_norm_backward", "vae_dense_aux_bytes", "vae_dense_forward", "vae_dense_workspace_floats", "vae_dense_backward",
+           "vae_layer_norm_backward", "vae_dense_aux_bytes", "vae_dense_forward", "vae_dense_forward_workspace_floats", "vae_dense_workspace_floats", "vae_dense_backward",
            "vae_gated_scan_kept_floats", "vae_gated_scan_workspace_floats", "vae_gated_scan_forward", "vae_gated_scan_backward")
 
 

@@ -5,8 +5,8 @@
 //
 // All three are C[m][n] = sum_k A(m, k) B(n, k), each operand stored either with k contiguous (x and W in the forward pass, dp in
 // dx) or with its row contiguous (W in dx; dp and x in dW).  Products run on the matrix cores, sums in fp32, in one of four
-// kernels: dense_rows_k (forward, up to 64 rows: bound by the weight's bytes), gemm_k (operands of any alignment and products too
-// small for 128 x 128 tiles: bound by latency), gemm_dma_k (the others: bound by the matrix cores and the clock that their power
+// kernels: dense_rows_k (forward of few rows: bound by the weight's bytes), gemm_k (operands of any alignment and products too
+// small for larger tiles: bound by latency), gemm_dma_k (the others: bound by the matrix cores and the clock that their power
 // leaves them), gemm_pair_k (dW and dx of a small layer in one launch).  Around the products of a backward pass stand a pass that makes
 // dp and its column sums (dense_dact_k: bytes) and one that adds the slices of dW and the partial sums of db (dense_join_k).
 #include <atomic>
@@ -306,13 +306,13 @@ __device__ __forceinline__ void tile_of(int tile, int M, int N, int BM, int BN, 
     m = grp * 8 + (in - n * h);
 }
 
-// C tile BM x BN by WM x WN waves, for products too small for the kernel below and for operands of any alignment.  The tiles of
+// C tile of 64 x 64 by four waves, for products too small for the kernel below and for operands of any alignment.  The tiles of
 // the operands pass registers, AHEAD of them in flight: with a workgroup or two a CU a tile's loads take longer than its products,
 // and only loads in flight hide that (256 x 4,096 x 4,096 bf16 forward: 46 us with one tile ahead, 29 with four).  The matrix instruction's first operand is B: a lane then
 // holds four neighbouring columns n of one row m of C.
-template <typename T, int BM, int BN, int WM, int WN, int AHEAD, bool ARC, bool BRC>
+template <typename T, bool ARC, bool BRC>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tile, int slice, char* lds) {
-    constexpr int NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int BM = 64, BN = 64, WM = 2, WN = 2, AHEAD = 4, NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int m0, n0;
     tile_of(tile, g.M, g.N, BM, BN, m0, n0);
@@ -365,18 +365,18 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tile, int slice
     __syncthreads();
     store_tile<T, FM, FN>(g, acc, m0 + wm, n0 + wn, slice, lane, reinterpret_cast<float*>(lds) + w * 32 * (FN * 16 + 4));
 }
-template <typename T, int B, int AHEAD, bool ARC, bool BRC>
+template <typename T, bool ARC, bool BRC>
 __global__ __launch_bounds__(256) void gemm_k(const GemmArgs g) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    gemm_tile<T, B, B, 2, 2, AHEAD, ARC, BRC>(g, blockIdx.x, blockIdx.z, lds);
+    gemm_tile<T, ARC, BRC>(g, blockIdx.x, blockIdx.z, lds);
 }
 // dW and dx of a small layer side by side: neither fills the chip, and a launch is saved.
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_pair_k(const GemmArgs dw, int dw_tiles, int dw_blocks, const GemmArgs dx) {
+__global__ __launch_bounds__(256) void gemm_pair_k(const GemmArgs dw, int dw_tiles, int dw_blocks, const GemmArgs dx, int dx_tiles) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    const int i = blockIdx.x;
-    if (i < dw_blocks) gemm_tile<T, 64, 64, 2, 2, 4, true, true>(dw, i % dw_tiles, i / dw_tiles, lds);
-    else gemm_tile<T, 64, 64, 2, 2, 4, false, true>(dx, i - dw_blocks, 0, lds);
+    const int i = blockIdx.x, j = i - dw_blocks;
+    if (j < 0) gemm_tile<T, true, true>(dw, i % dw_tiles, i / dw_tiles, lds);
+    else gemm_tile<T, false, true>(dx, j % dx_tiles, j / dx_tiles, lds);
 }
 
 // ---- The large products -----------------------------------------------------------------------------------------------
@@ -532,11 +532,15 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
 }
 
 // ---- Few rows (serving) --------------------------------------------------------------------------------------------------
-// y of up to 64 rows: the weight's bytes are the bound, so they are read once and straight into registers.  A workgroup takes 16
+// y of few rows: the weight's bytes are the bound, so they are read once and straight into registers.  A workgroup takes 16
 // columns of y (rows of w) and shares k out among its waves; each wave has eight 1-KiB loads in flight, multiplies them on the matrix
 // cores with MF x 16 rows of x (zeros where there are fewer), and the waves' sums meet in LDS.  4,096 x 4,096 bf16, one row: 11 us a
-// call (a third of it launch; 33.6 MB would take 6.6).  Up to 64 rows, as the tiles of gemm_k are 64 high: less would be padding there.
-constexpr int ROWS_MAX = 64, ROWS_STEPS = 8;
+// call (a third of it launch; 33.6 MB would take 6.6).
+//   Few are 32, and 64 where eight waves have all of k in flight: 48 rows of 4,096 x 512 fp32 take 9 us here and 14 in tiles of gemm_k,
+// of 1,024 x 1,024 12 and 14, of 2,048 x 2,048 23 and 14; bf16: of 2,048 x 2,048 10 and 13, of 512 x 4,096 17 and 13; 32 rows of 4,096 x 4,096
+// bf16 14 and 16.
+constexpr int ROWS_STEPS = 8;
+bool dense_few(int64_t M, int64_t K, int es) { return M <= 32 || (M <= 64 && K * es <= 8 * ROWS_STEPS * 64); }
 template <typename T, int MF>
 __global__ __launch_bounds__(MF == 4 ? 512 : 1024) void dense_rows_k(const GemmArgs g, int steps) {  // steps: pieces of 64 bytes of k a wave takes
     constexpr int V = 16 / sizeof(T), KS = 4 * V;
@@ -596,32 +600,40 @@ int dense_rows(const GemmArgs& g, hipStream_t s) {
     constexpr int KS = 64 / sizeof(T);
     const int pieces = (int)ceil_div64(g.K, KS);
     int waves = (int)ceil_div64(pieces, ROWS_STEPS);
-    if (waves > (g.M > 32 ? 8 : 16)) waves = g.M > 32 ? 8 : 16;
+    if (waves > 16) waves = 16;
     const int steps = (int)ceil_div64(pieces, waves);
     const dim3 grid((unsigned)ceil_div64(g.N, 16)), block(waves * 64);
     if (g.M <= 16) dense_rows_k<T, 1><<<grid, block, 0, s>>>(g, steps);
     else if (g.M <= 32) dense_rows_k<T, 2><<<grid, block, 0, s>>>(g, steps);
-    else dense_rows_k<T, 4><<<grid, block, 0, s>>>(g, steps);
+    else dense_rows_k<T, 4><<<grid, block, 0, s>>>(g, steps);  // (eight waves at most: dense_few)
     VAE_LAUNCH_CHECK("dense_rows_k");
     return VAE_OK;
 }
 
-// What the backward pass leaves in parts, added in a fixed order: the first join_blocks workgroups add the slices of dW (1024 values
-// each), the others the rows of db's partial sums (64 columns each, four waves that take every fourth row).
+// What the backward pass leaves in parts, added in a fixed order: the first workgroups add the slices of dW (1024 values each),
+// then those of dx, the others the rows of db's partial sums (64 columns each, four waves that take every fourth row).
 template <typename T>
-__global__ __launch_bounds__(256) void dense_join_k(const float* part, int slices, int64_t n, T* c, int join_blocks, const float* cols, int rows,
-                                                    int N, T* db) {
-    if ((int)blockIdx.x < join_blocks) {
-        const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-        if (i >= n) return;
+struct Slices {
+    const float* part;  // [slices][n]
+    int64_t n;
+    T* out;
+    int slices, blocks;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void dense_join_k(const Slices<T> dw, const Slices<T> dx, const float* cols, int rows, int N, T* db) {
+    const int b = (int)blockIdx.x - dw.blocks, join_blocks = dw.blocks + dx.blocks;
+    if (b < dx.blocks) {
+        const Slices<T>& j = b < 0 ? dw : dx;
+        const int64_t i = ((int64_t)(b < 0 ? (int)blockIdx.x : b) * 256 + threadIdx.x) * 4;
+        if (i >= j.n) return;
         float s[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
 #pragma unroll 4
-        for (int k = 0; k < slices; ++k) {
-            load_part<float, 4>(v, part + k * n + i, n - i);
+        for (int k = 0; k < j.slices; ++k) {
+            load_part<float, 4>(v, j.part + k * j.n + i, j.n - i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[e] += v[e];
         }
-        store_part<T, 4>(c + i, s, n - i);
+        store_part<T, 4>(j.out + i, s, j.n - i);
         return;
     }
     __shared__ float red[4][64];
@@ -634,6 +646,37 @@ __global__ __launch_bounds__(256) void dense_join_k(const float* part, int slice
     red[w][lane] = s;
     __syncthreads();
     if (w == 0 && col < N) db[col] = (T)(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
+}
+
+// ... and the forward pass: a lane adds 8 neighbouring values and gives them the epilogue that a whole product has in store_tile.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_ends_k(const GemmArgs g, int slices) {
+    const int per = (g.N + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / per;
+    if (m >= g.M) return;
+    const int n = (int)(i - m * per) * 8, left = g.N - n;
+    float v[8], p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < slices; ++k) {
+        load_part<float, 8>(p, g.part + ((int64_t)k * g.M + m) * g.N + n, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p[e];
+    }
+    if (g.bias != nullptr) {
+        load_part<T, 8>(p, (const T*)g.bias + n, left);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p[e];
+    }
+    if (g.aux != nullptr) aux_store8(g.aux, m * g.N + n, v, g.auxk, left);
+    dense_act8<sizeof(T) == 2>(v, g.act, g.slope);
+    if (g.res != nullptr) {
+        load_part<T, 8>(p, (const T*)g.res + m * g.ldr + n, left, g.N >= 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p[e];
+    }
+    store_part<T, 8>((T*)g.c + m * g.ldc + n, v, left);
 }
 
 // dp = dy act'(p), rounded to the type of the products that read it (the matrix cores take their operands so), and the column sums
@@ -686,13 +729,13 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
     part[(int64_t)blockIdx.y * N + at] = t;
 }
 
-template <typename T, int BM, int BN, bool ARC, bool BRC, bool DMA>
+template <typename T, int B, bool ARC, bool BRC>
 int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
-    constexpr int bytes = 2 * (BM + BN) * KB;
-    static_assert(4 * 32 * (BN / 2 + 4) * 4 <= bytes && BM == BN, "the epilogue's LDS");
+    constexpr int bytes = 4 * B * KB;
+    static_assert(4 * 32 * (B / 2 + 4) * 4 <= bytes, "the epilogue's LDS");
     void (*k)(const GemmArgs);
-    if constexpr (DMA) k = gemm_dma_k<T, BM, BN, ARC, BRC>;
-    else k = gemm_k<T, BM, BM == 64 ? 4 : 2, ARC, BRC>;
+    if constexpr (B == 64) k = gemm_k<T, ARC, BRC>;
+    else k = gemm_dma_k<T, B, B, ARC, BRC>;
     if (bytes > 65536) {
         static std::atomic<uint64_t> granted{0};  // a bit a device (two threads at once both ask, which does no harm)
         int dev = 0;
@@ -702,17 +745,12 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
             if (dev < 64) granted.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
         }
     }
-    const int64_t tiles = ceil_div64(g.N, BN) * ceil_div64(g.M, BM);
+    const int64_t tiles = ceil_div64(g.N, B) * ceil_div64(g.M, B);
     if (tiles > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "gemm: %lld tiles", (long long)tiles);
     k<<<dim3((unsigned)tiles, 1, slices), dim3(256), bytes, s>>>(g);
     VAE_LAUNCH_CHECK("gemm_k");
     return VAE_OK;
 }
-
-// Tile of the product: 128 x 128, or 64 x 64 where those give too few workgroups.
-bool gemm_small(int64_t M, int64_t N) { return ceil_div64(M, 128) * ceil_div64(N, 128) < 256; }
-
-bool gemm_large(int64_t M, int64_t N) { return ceil_div64(M, 256) * ceil_div64(N, 256) >= 192; }
 
 // Can the operands go to LDS directly: rows that start and end on 16 bytes, a tile's rows within 31 bits of offset.
 template <typename T>
@@ -723,28 +761,63 @@ bool whole_pieces(const GemmArgs& g, bool arc, bool brc) {
            (brc ? g.N : g.K) % V == 0 && g.lda < most && g.ldb < most;
 }
 
-// Slices of k of a split product (the weight gradient: few outputs, a long sum): enough workgroups for the chip, at least 8
-// k-tiles each.
-int gemm_slices(int64_t M, int64_t N, int64_t K, int bk, int* kslice) {
-    const int t = gemm_small(M, N) ? 64 : 128;
-    const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t), kt = ceil_div64(K, bk);
-    int64_t s = tiles >= 256 ? 1 : ceil_div64(512, tiles);
-    if (s > kt / 8) s = kt / 8;
-    if (s < 1) s = 1;
-    const int64_t per = ceil_div64(kt, s);
-    *kslice = (int)(per * bk);
-    return (int)ceil_div64(kt, per);
+// Tile and slices of k of a product: the pair that takes least by what was measured of each.  256 workgroups at a time, one a CU,
+// take TILE_US[][0] and [1] a k-tile of 128 bytes; slices cost a launch more and their way through memory.  Operands that are not
+// whole pieces take tiles of 64 (register-staged ones of 128 measured 33 us against 22 for 1,537 x 1,001 x 1,283 fp16, and the same for
+// fp32).
+//   16-bit types, us: 2,048 x 1,024 x 2,048 19 (tiles of 64), 24 (128); 2,048 x 1,920 x 2,048 30 (64), 23 (128); 4,096 x 2,048 x 4,096 79
+// (128), 97 (256); 4,096 x 2,816 x 4,096 107 (128), 97 (256).  fp32: 2,048 x 1,536 x 2,048 113 (64), 139 (128); 2,048 x 2,304 x 2,048 185 (64),
+// 245 (128).  Split: 65 x 4,096 x 4,096 bf16 25 whole, 16 in slices; fp32 90, 45.
+struct GemmPlan {
+    int tile, slices, kslice;
+};
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int es, bool whole) {
+    constexpr float TILE_US[2][3][2] = {{{1.f, 0.30f}, {8.f, 0.457f}, {22.5f, 1.16f}}, {{1.5f, 0.58f}, {8.f, 2.f}, {0.f, 0.f}}};  // 16-bit, fp32: 64, 128, 256
+    const int64_t bk = KB / es, kt = ceil_div64(K, bk);
+    GemmPlan best = {};
+    float least = 0.f;
+    for (int i = 0; i < (!whole ? 1 : es == 2 ? 3 : 2); ++i) {
+        const int t = 64 << i;
+        const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t);
+        const float* c = TILE_US[es == 4][i];
+        for (int rounds = 0; rounds <= 2; ++rounds) {  // (0: not split)
+            int64_t s = 1;
+            if (rounds > 0) {
+                s = rounds * 256 / tiles;
+                if (s > kt / 8) s = kt / 8;  // (at least 8 k-tiles a slice)
+                if (s < 2) continue;
+            }
+            const int64_t per = ceil_div64(kt, s);
+            s = ceil_div64(kt, per);
+            const int64_t turns = ceil_div64(tiles * s, 256);
+            float us = (float)turns * (c[0] + (float)per * c[1]);
+            if (turns == 1 && t < 256) us *= 1.15f;  // (a CU takes two of these tiles at once, and is better busy then)
+            if (s > 1) us += 5.f + 2e-6f * (float)s * (float)M * (float)N;
+            if (best.tile == 0 || us < least) least = us, best = {t, (int)s, (int)(per * bk)};
+        }
+    }
+    if (best.slices == 1) best.kslice = (int)K;
+    return best;
+}
+template <typename T>
+GemmPlan gemm_plan(const GemmArgs& g, bool arc, bool brc) {
+    return gemm_plan(g.M, g.N, g.K, sizeof(T), whole_pieces<T>(g, arc, brc));
+}
+// floats that the slices take at most, wherever the operands lie
+int64_t gemm_split_floats(int64_t M, int64_t N, int64_t K, int es) {
+    const int a = gemm_plan(M, N, K, es, false).slices, b = gemm_plan(M, N, K, es, true).slices, s = a > b ? a : b;
+    return s > 1 ? s * M * N : 0;
 }
 
 // slices > 1: g.part holds the sums, the caller adds them up
 template <typename T, bool ARC, bool BRC>
-int gemm(const GemmArgs& g, int slices, hipStream_t s) {
-    if (gemm_small(g.M, g.N)) return gemm_inst<T, 64, 64, ARC, BRC, false>(g, slices, s);
-    if (!whole_pieces<T>(g, ARC, BRC)) return gemm_inst<T, 128, 128, ARC, BRC, false>(g, slices, s);
+int gemm(GemmArgs g, const GemmPlan& p, hipStream_t s) {
+    g.kslice = p.kslice;
+    if (p.tile == 64) return gemm_inst<T, 64, ARC, BRC>(g, p.slices, s);
     if constexpr (sizeof(T) == 2) {
-        if (gemm_large(g.M, g.N)) return gemm_inst<T, 256, 256, ARC, BRC, true>(g, slices, s);
+        if (p.tile == 256) return gemm_inst<T, 256, ARC, BRC>(g, p.slices, s);
     }
-    return gemm_inst<T, 128, 128, ARC, BRC, true>(g, slices, s);
+    return gemm_inst<T, 128, ARC, BRC>(g, p.slices, s);
 }
 
 // Slices of the rows: about 2048 workgroups in all, 256 at most (rows of partial sums)
@@ -760,19 +833,34 @@ int dact_rows(int64_t M, int64_t N) {
 int64_t dp_stride(int64_t N, int es) { return ceil_div64(N, 16 / es) * (16 / es); }
 
 struct DenseWs {  // workspace of the backward pass, in floats
-    int64_t dp, split, cols, total;
+    int64_t dp, split_w, split_x, cols, total;
 };
 DenseWs dense_ws(int64_t M, int64_t N, int64_t K, int dtype, int act) {
-    DenseWs w;
+    DenseWs l;
     const int es = vae_type_size(dtype);
     const int64_t a = 64;
-    w.dp = 0;
-    w.split = w.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * dp_stride(N, es) * es, 4), a) * a);
-    int ks;
-    const int s = gemm_slices(N, K, M, KB / es, &ks);
-    w.cols = w.split + (s > 1 ? ceil_div64((int64_t)s * N * K, a) * a : 0);
-    w.total = w.cols + dact_rows(M, N) * N;
-    return w;
+    l.dp = 0;
+    l.split_w = l.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * dp_stride(N, es) * es, 4), a) * a);
+    l.split_x = l.split_w + ceil_div64(gemm_split_floats(N, K, M, es), a) * a;
+    l.cols = l.split_x + ceil_div64(gemm_split_floats(M, K, N, es), a) * a;
+    l.total = l.cols + dact_rows(M, N) * N;
+    return l;
+}
+
+template <typename T>
+int dense_forward_t(GemmArgs& g, float* workspace, hipStream_t s) {
+    if (dense_few(g.M, g.K, sizeof(T))) return dense_rows<T>(g, s);
+    const GemmPlan p = gemm_plan<T>(g, false, false);
+    if (p.slices > 1) {
+        if (workspace == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null workspace");
+        g.part = workspace;
+    }
+    if (int rc = gemm<T, false, false>(g, p, s)) return rc;
+    if (p.slices > 1) {
+        dense_ends_k<T><<<dim3((unsigned)ceil_div64((int64_t)g.M * ((g.N + 7) / 8), 256)), dim3(256), 0, s>>>(g, p.slices);
+        VAE_LAUNCH_CHECK("dense_ends_k");
+    }
+    return VAE_OK;
 }
 
 template <typename T>
@@ -790,23 +878,26 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
         if (auxk != AUX_NONE) dp = out, lddp = dp_stride(N, sizeof(T));
     }
     GemmArgs gx = {}, gw = {};
-    gx.a = dp, gx.lda = lddp, gx.b = w, gx.ldb = ldw, gx.c = dx, gx.ldc = K, gx.M = M, gx.N = K, gx.K = N, gx.kslice = N;
+    gx.a = dp, gx.lda = lddp, gx.b = w, gx.ldb = ldw, gx.c = dx, gx.ldc = K, gx.M = M, gx.N = K, gx.K = N;
     gw.a = dp, gw.lda = lddp, gw.b = x, gw.ldb = ldx, gw.c = dw, gw.ldc = K, gw.M = N, gw.N = K, gw.K = M;
-    const int slices = gemm_slices(N, K, M, BK<T>(), &gw.kslice);
-    if (slices > 1) gw.part = ws + lay.split;
-    const int64_t tx = ceil_div64(M, 64) * ceil_div64(K, 64), tw = ceil_div64(N, 64) * ceil_div64(K, 64);
-    if (dx != nullptr && dw != nullptr && gemm_small(M, K) && gemm_small(N, K)) {
-        gemm_pair_k<T><<<dim3((unsigned)(tw * slices + tx)), dim3(256), 2 * 128 * KB, s>>>(gw, (int)tw, (int)(tw * slices), gx);
+    const GemmPlan pw = gemm_plan<T>(gw, true, true), px = gemm_plan<T>(gx, false, true);
+    Slices<T> jw = {ws + lay.split_w, (int64_t)N * K, dw, pw.slices, 0}, jx = {ws + lay.split_x, (int64_t)M * K, dx, px.slices, 0};
+    if (dw != nullptr && jw.slices > 1) gw.part = ws + lay.split_w, jw.blocks = (int)ceil_div64(jw.n, 1024);
+    if (dx != nullptr && jx.slices > 1) gx.part = ws + lay.split_x, jx.blocks = (int)ceil_div64(jx.n, 1024);
+    if (dx != nullptr && dw != nullptr && pw.tile == 64 && px.tile == 64) {
+        const int tw = (int)(ceil_div64(N, 64) * ceil_div64(K, 64)), tx = (int)(ceil_div64(M, 64) * ceil_div64(K, 64));
+        gw.kslice = pw.kslice, gx.kslice = px.kslice;
+        gemm_pair_k<T><<<dim3((unsigned)(tw * jw.slices + tx * jx.slices)), dim3(256), 2 * 128 * KB, s>>>(gw, tw, tw * jw.slices, gx, tx);
         VAE_LAUNCH_CHECK("gemm_pair_k");
     } else {
         if (dx != nullptr)
-            if (int rc = gemm<T, false, true>(gx, 1, s)) return rc;
+            if (int rc = gemm<T, false, true>(gx, px, s)) return rc;
         if (dw != nullptr)
-            if (int rc = gemm<T, true, true>(gw, slices, s)) return rc;
+            if (int rc = gemm<T, true, true>(gw, pw, s)) return rc;
     }
-    const int64_t n = (int64_t)N * K, join = dw != nullptr && slices > 1 ? ceil_div64(n, 1024) : 0, sums = db != nullptr ? ceil_div64(N, 64) : 0;
-    if (join + sums > 0) {
-        dense_join_k<T><<<dim3((unsigned)(join + sums)), dim3(256), 0, s>>>(ws + lay.split, slices, n, dw, (int)join, ws + lay.cols, ny, N, db);
+    const int64_t sums = db != nullptr ? ceil_div64(N, 64) : 0;
+    if (jw.blocks + jx.blocks + sums > 0) {
+        dense_join_k<T><<<dim3((unsigned)(jw.blocks + jx.blocks + sums)), dim3(256), 0, s>>>(jw, jx, ws + lay.cols, ny, N, db);
         VAE_LAUNCH_CHECK("dense_join_k");
     }
     return VAE_OK;
@@ -827,7 +918,7 @@ extern "C" int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype)
 }
 
 extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
-                                 void* y, int64_t ldy, void* aux, int M, int N, int K, int act, float slope, int dtype,
+                                 void* y, int64_t ldy, void* aux, float* workspace, int M, int N, int K, int act, float slope, int dtype,
                                  vae_stream_t stream) {
     if (int rc = dense_check("dense_forward", M, N, K, act, dtype)) return rc;
     if (M == 0) return VAE_OK;
@@ -838,11 +929,14 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.c = y, g.ldc = ldy, g.bias = bias, g.res = res, g.ldr = ldr;
     g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
     g.aux = g.auxk == AUX_NONE ? nullptr : aux;
-    g.kslice = K;
     hipStream_t s = (hipStream_t)stream;
-    if (M <= ROWS_MAX) return dtype == VAE_T_F32 ? dense_rows<float>(g, s) : dtype == VAE_T_BF16 ? dense_rows<bf16_t>(g, s) : dense_rows<f16_t>(g, s);
-    if (dtype == VAE_T_F32) return gemm<float, false, false>(g, 1, s);
-    return dtype == VAE_T_BF16 ? gemm<bf16_t, false, false>(g, 1, s) : gemm<f16_t, false, false>(g, 1, s);
+    if (dtype == VAE_T_F32) return dense_forward_t<float>(g, workspace, s);
+    return dtype == VAE_T_BF16 ? dense_forward_t<bf16_t>(g, workspace, s) : dense_forward_t<f16_t>(g, workspace, s);
+}
+
+extern "C" int64_t vae_dense_forward_workspace_floats(int64_t M, int64_t N, int64_t K, int dtype) {
+    if (M < 1 || N < 1 || K < 1 || vae_type_size(dtype) == 0 || dense_few(M, K, vae_type_size(dtype))) return 0;
+    return gemm_split_floats(M, N, K, vae_type_size(dtype));
 }
 
 extern "C" int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype) {

@@ -153,8 +153,12 @@ def _linear_forward(x, weight, bias, act, slope, residual, device, code, save):
         lib = L.lib()
         if save and act != L.ACT_NONE:
             aux = xr.new_empty(lib.vae_dense_aux_bytes(M, N, act, code), dtype=torch.uint8)
+        ws = None
+        if M > 1:  # (a served model's one token skips the question)
+            n = lib.vae_dense_forward_workspace_floats(M, N, K, code)
+            ws = xr.new_empty(n, dtype=torch.float32) if n else None
         _call(lib.vae_dense_forward, "vae_dense_forward", device, xr.data_ptr(), ldx, wr.data_ptr(), ldw, _p(bias), _p(rr), ldr,
-              y.data_ptr(), N, _p(aux), M, N, K, act, slope, code)
+              y.data_ptr(), N, _p(aux), _p(ws), M, N, K, act, slope, code)
     return y, xr, wr, aux, (M, N, K, ldx, ldw, act, slope, device, code)
 
 
