@@ -105,6 +105,15 @@ def test_norm_values_and_gradients(rows, cols, dtype):
             check(k, got[k], v, tol)
 
 
+@pytest.mark.parametrize("rows,cols", [(600, 8200), (4, 12288), (300, 12291), (3, 16384)])
+def test_norm_rows_of_a_whole_workgroup(rows, cols):
+    x, dy = rnd((rows, cols), torch.float32, 1, 1.5, 0.3), rnd((rows, cols), torch.float32, 2)
+    w, b = rnd(cols, torch.float32, 3, 0.2, 1.0), rnd(cols, torch.float32, 4, 0.1)
+    got, want = run_norm(x, w, b, dy), norm64(x, w, b, dy, 1e-5)
+    for k, (v, tol) in want.items():
+        check(k, got[k], v, tol)
+
+
 @pytest.mark.parametrize("has_w,has_b", [(False, False), (True, False), (False, True)])
 def test_norm_without_parameters(has_w, has_b):
     x, dy = rnd((37, 200), torch.bfloat16, 1), rnd((37, 200), torch.bfloat16, 2)
