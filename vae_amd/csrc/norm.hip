@@ -406,17 +406,22 @@ int bwd_inst(const NormArgs& a) {
 
 constexpr int NORM_LONG_SLICES = 64;
 
-// The smallest group that holds the row: G lanes x NCH pieces of 16 bytes, all but the last of them full.
+// G lanes x NCH pieces of 16 bytes that hold the row, all pieces but the last of them full.  Two pieces a lane rather than one in
+// twice the lanes: half the shuffles and more bytes in flight a lane (134 MB of bf16, forward and backward: 524,288 x 128 48 -> 43 and 94 ->
+// 79 us, 131,072 x 512 47 -> 43 and 89 -> 78, 32,768 x 2,048 51 -> 41 and 93 -> 83); beyond 256 pieces the backward pass is better off with
+// one (16,384 x 4,096: 88, 99 with two).
 template <typename T, typename TW>
 int norm_forward_t(const NormArgs& a) {
     constexpr int V = 16 / sizeof(T);
     const int p = (a.C + V - 1) / V;  // 16-byte pieces of a row
-    if (p <= 8) return fwd_inst<T, TW, 8, 1>(a);
-    if (p <= 16) return fwd_inst<T, TW, 16, 1>(a);
-    if (p <= 32) return fwd_inst<T, TW, 32, 1>(a);
-    if (p <= 64) return fwd_inst<T, TW, 64, 1>(a);
+    if (p <= 4) return fwd_inst<T, TW, 4, 1>(a);
+    if (p <= 8) return fwd_inst<T, TW, 4, 2>(a);
+    if (p <= 16) return fwd_inst<T, TW, 8, 2>(a);
+    if (p <= 32) return fwd_inst<T, TW, 16, 2>(a);
+    if (p <= 64) return fwd_inst<T, TW, 32, 2>(a);
     if (p <= 128) return fwd_inst<T, TW, 64, 2>(a);
-    if (p <= 256) return fwd_inst<T, TW, 256, 1>(a);
+    if (p <= 192) return fwd_inst<T, TW, 64, 3>(a);
+    if (p <= 256) return fwd_inst<T, TW, 64, 4>(a);
     if (p <= 512) return fwd_inst<T, TW, 256, 2>(a);
     if (p <= 768) return fwd_inst<T, TW, 256, 3>(a);
     if (p <= 1024) return fwd_inst<T, TW, 512, 2>(a);
@@ -436,12 +441,16 @@ template <typename T, typename TW>
 int norm_backward_t(const NormArgs& a) {
     constexpr int V = 16 / sizeof(T);
     const int p = (a.C + V - 1) / V;
-    if (p <= 8) return bwd_inst<T, TW, 8, 1>(a);
-    if (p <= 16) return bwd_inst<T, TW, 16, 1>(a);
-    if (p <= 32) return bwd_inst<T, TW, 32, 1>(a);
-    if (p <= 64) return bwd_inst<T, TW, 64, 1>(a);
+    if (p <= 4) return bwd_inst<T, TW, 4, 1>(a);
+    if constexpr (sizeof(T) == 4) {  // (30 columns: 84 us, 92 with 4 x 2)
+        if (p <= 8) return bwd_inst<T, TW, 8, 1>(a);
+    }
+    if (p <= 8) return bwd_inst<T, TW, 4, 2>(a);
+    if (p <= 16) return bwd_inst<T, TW, 8, 2>(a);
+    if (p <= 32) return bwd_inst<T, TW, 16, 2>(a);
+    if (p <= 64) return bwd_inst<T, TW, 32, 2>(a);
     if (p <= 128) return bwd_inst<T, TW, 64, 2>(a);
-    if (p <= 256) return bwd_inst<T, TW, 256, 1>(a);
+    if (p <= 256) return bwd_inst<T, TW, 128, 2>(a);
     if (p <= 512) return bwd_inst<T, TW, 512, 1>(a);
     if (p <= 1024) return bwd_inst<T, TW, 1024, 1>(a);
     if (p <= 1536) return bwd_inst<T, TW, 512, 3>(a);
