@@ -427,25 +427,34 @@ __global__ __launch_bounds__(64) void gscan_step_k(const GsArgs a) {
 
 int64_t gs_columns(int B, int D, int V) { return ceil_div64((int64_t)B * ((D + V - 1) / V), 64); }
 
-// What a launch looks like: V features a lane (as many as leave 256 columns of workgroups; at most 8 bytes forward, 8 and 4 bytes
-// (fp32 and 16-bit types) backward, where more would not stay in registers; never more than D), W waves a workgroup, parts of the
-// time axis, as many as make 512 workgroups.  Parts read x and gate (backward: gate and dy) twice, but let more workgroups at them than
-// the channels make.  In parts and in one go, T = 4,096: fp32 forward 31 and 62 us at 24 columns, 60 and 62 at 64, 70 and 63 at 72 (T =
-// 16,384: 266 and 307 at 64, 331 and 333 at 80), backward 161 and 164 at 104, 191 and 181 at 128; bf16 forward 43 and 61 at 64, 53 and
-// 61 at 80, 63 and 61 at 88, backward 106 and 137 at 128, 137 and 131 at 144.  Below four tiles there is little to share out (T = 512
-// forward: 14 and 10).
+// What a launch looks like.  V features a lane: as many as leave 256 columns of workgroups, at most 8 bytes forward and 8 and 4 bytes
+// (fp32 and 16-bit types) backward, where more would not stay in registers; never more than D, and four only where a row holds whole fours
+// (1,000 x 1,000 x 67 bf16: 140 us, 173 with fours across the rows' ends).
+//   W waves a workgroup: as few as hold a short series, or (forward; the backward pass starts from states 64 steps apart) most of its
+// last tile: 4,096 x 9 x 1,800 fp32 162 us with two, 250 with four; 1,024 x 65 x 1,000 bf16 100 with four, 154 with eight.  16 for a long
+// series while each column of channels has a CU of its own, 8 beyond: 8 x 1,024 x 2,304 bf16 31 us forward and 58 backward, 36 and 64 with
+// 16 (four for V of 2 and 4 would cost up to a fifth of the backward pass).
+//   Parts of the time axis: as many as make 512 workgroups.  They read x and gate (backward: gate and dy) twice, but let more workgroups
+// at them than the channels make.  In parts and in one go, T = 4,096: fp32 forward 31 and 62 us at 24 columns, 60 and 62 at 64, 70 and 63
+// at 72 (T = 16,384: 266 and 307 at 64, 331 and 333 at 80), backward 161 and 164 at 104, 191 and 181 at 128; bf16 forward 43 and 61 at
+// 64, 53 and 61 at 80, 63 and 61 at 88, backward 106 and 137 at 128, 137 and 131 at 144.  Below four tiles there is little to share
+// out (T = 512 forward: 14 and 10).
 struct GsPlan {
     int V, W, parts, part_steps;
 };
 GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
     GsPlan p;
     p.V = esize == 2 && fwd ? 4 : 2;
+    if (p.V == 4 && D % 4 != 0) p.V = 2;
     while (p.V > 1 && (p.V > D || gs_columns(B, D, p.V) < 256)) p.V >>= 1;
     const int64_t cols = gs_columns(B, D, p.V);
-    p.W = T <= GS_S ? 1 : T <= 4 * GS_S ? 4 : cols >= 512 || T <= GS_TILE || p.V > 1 ? 8 : 16;
+    if (T <= GS_S) p.W = 1;
+    else if (T <= 2 * GS_S) p.W = 2;
+    else if (T <= 4 * GS_S || (fwd && T < 256 && (T - 1) % GS_TILE < GS_TILE / 2)) p.W = 4;
+    else p.W = T <= GS_TILE || p.V > 1 || cols > 256 ? 8 : 16;
     const int64_t tile = p.W * (fwd ? gs_steps(p.W) : GS_S), tiles = ceil_div64(T, tile);
     const int64_t enough = fwd ? (esize == 4 ? 72 : 88) : (esize == 4 ? 112 : 136);
-    int64_t n = cols >= enough || tiles < 4 ? 1 : 512 / cols;
+    int64_t n = p.W < 16 || cols >= enough || tiles < 4 ? 1 : 512 / cols;
     if (n > GS_MAX_PARTS) n = GS_MAX_PARTS;
     if (n > tiles) n = tiles;
     const int64_t per = ceil_div64(tiles, n);
@@ -457,7 +466,7 @@ GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
 template <typename T, int V, int W, bool FWD>
 int gs_launch(const GsArgs& a) {
     const dim3 grid((unsigned)gs_columns(a.B, a.D, V), a.parts);
-    if constexpr (W == 16) {  // (fewer waves: a short series, or channels enough)
+    if constexpr (W == 16) {
         if (a.parts > 1) {
             if (FWD) gscan_fwd_k<T, V, W, gs_steps(W), true><<<grid, dim3(W * 64), 0, a.s>>>(a);
             else gscan_bwd_k<T, V, W, true><<<grid, dim3(W * 64), 0, a.s>>>(a);
@@ -479,6 +488,7 @@ int gs_run(GsArgs& a) {
 #define VAE_GS(NV)                                                      \
     if (p.V == NV) {                                                    \
         if (p.W == 1) return gs_launch<T, NV, 1, FWD>(a);               \
+        if (p.W == 2) return gs_launch<T, NV, 2, FWD>(a);               \
         if (p.W == 4) return gs_launch<T, NV, 4, FWD>(a);               \
         if (p.W == 8) return gs_launch<T, NV, 8, FWD>(a);               \
         if constexpr (NV == 1) return gs_launch<T, 1, 16, FWD>(a);      \
