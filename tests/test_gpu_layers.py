@@ -105,7 +105,7 @@ def test_norm_values_and_gradients(rows, cols, dtype):
             check(k, got[k], v, tol)
 
 
-@pytest.mark.parametrize("rows,cols", [(600, 8200), (4, 12288), (300, 12291), (3, 16384)])
+@pytest.mark.parametrize("rows,cols", [(600, 8200), (4, 12288), (300, 12291), (3, 16384), (300, 18801), (300, 18838), (300, 18843)])
 def test_norm_rows_of_a_whole_workgroup(rows, cols):
     x, dy = rnd((rows, cols), torch.float32, 1, 1.5, 0.3), rnd((rows, cols), torch.float32, 2)
     w, b = rnd(cols, torch.float32, 3, 0.2, 1.0), rnd(cols, torch.float32, 4, 0.1)

@@ -15,6 +15,25 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
+// p moved down by n of its bytes (multiples of T), zeros behind.  In 32-bit steps: a 64-bit shift by a register gave wrong results here
+// when that register was the last one that the kernel had (v31 of 32; some waves, some runs).
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> shift_down(const Pack<T, N>& p, int n) {
+    constexpr int D = N * sizeof(T) / 4;
+    struct Dwords {
+        uint32_t d[D];
+    } q = __builtin_bit_cast(Dwords, p);
+#pragma unroll
+    for (int step = D / 2; step >= 1; step >>= 1)
+#pragma unroll
+        for (int i = 0; i < D; ++i) q.d[i] = n & (step * 4) ? (i + step < D ? q.d[i + step] : 0u) : q.d[i];
+    if constexpr (sizeof(T) < 4) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) q.d[i] = __builtin_amdgcn_alignbit(i + 1 < D ? q.d[i + 1] : 0u, q.d[i], (n & 3) * 8);
+    }
+    return __builtin_bit_cast(Pack<T, N>, q);
+}
+
 // `left` of the N elements at p (the others are 0 and are not read), as they are in memory.  wide: the row that they end has N
 // elements or more; then its last N are read in one piece and shifted into place (element by element it takes N - 1 loads).
 template <typename T, int N>
@@ -29,16 +48,7 @@ __device__ __forceinline__ void load_raw(Pack<T, N>& r, const T* p, int64_t left
     if constexpr (N * sizeof(T) == 16 || N * sizeof(T) == 8) {
         if (wide) {
             r = *reinterpret_cast<const Pack<T, N>*>(p - (N - (int)left));
-            const int sh = (N - (int)left) * (int)sizeof(T) * 8;
-            if constexpr (N * sizeof(T) == 8) {
-                r = __builtin_bit_cast(Pack<T, N>, __builtin_bit_cast(uint64_t, r) >> sh);
-            } else {
-                struct Two { uint64_t lo, hi; };
-                Two t = __builtin_bit_cast(Two, r);
-                t.lo = sh < 64 ? t.lo >> sh | t.hi << (64 - sh) : t.hi >> (sh - 64);
-                t.hi = sh < 64 ? t.hi >> sh : 0;
-                r = __builtin_bit_cast(Pack<T, N>, t);
-            }
+            r = shift_down(r, (N - (int)left) * (int)sizeof(T));
             return;
         }
     }
