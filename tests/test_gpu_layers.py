@@ -768,3 +768,62 @@ def test_refusals():
     (g,) = torch.autograd.grad((layers.layer_norm(xg) * xg).sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):  # differentiable once
         g.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------------ beyond 2^31 elements
+def _long(*shape):
+    t = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
+    assert t.numel() > 2 ** 31
+    for part in t.view(-1).split(2 ** 28):
+        part.normal_()
+    return t
+
+
+def test_norm_beyond_32_bits_of_offset():
+    """The last rows of a tensor of 2.2e9 elements, alone in having a gradient."""
+    from vae_amd import layers
+    rows, cols, n = 2_000_001, 1100, 40
+    x = _long(rows, cols).requires_grad_()
+    w, b = rnd(cols, torch.float32, 3, 0.2, 1.0).requires_grad_(), rnd(cols, torch.float32, 4, 0.1).requires_grad_()
+    y = layers.layer_norm(x, w, b)
+    dy = torch.zeros_like(y)
+    dy[-n:] = rnd((n, cols), torch.bfloat16, 5)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    want = norm64(x.detach()[-n:], w.detach(), b.detach(), dy[-n:], 1e-5)
+    for name, got in (("y", y.detach()[-n:]), ("dx", dx[-n:]), ("dw", dw), ("db", db)):
+        check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("m,n,k", [(1_048_616, 24, 2104), (1_048_616, 24, 2101), (262_184, 8200, 64)])
+def test_linear_beyond_32_bits_of_offset(m, n, k):
+    """x, then y, of more than 2^31 elements: as above."""
+    from vae_amd import layers
+    last = 40
+    x = (_long(m, k) if m * k > 2 ** 31 else rnd((m, k), torch.bfloat16, 1)).requires_grad_()
+    w = rnd((n, k), torch.bfloat16, 2, k ** -0.5).requires_grad_()
+    y = layers.linear(x, w, act="leaky", slope=SLOPE)
+    dy = torch.zeros_like(y)
+    dy[-last:] = rnd((last, n), torch.bfloat16, 5)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want = linear64(x.detach()[-last:], w.detach(), None, None, dy[-last:], "leaky")
+    for name, got in (("y", y.detach()[-last:]), ("dx", dx[-last:]), ("dw", dw)):
+        check(name, got, *want[name])
+
+
+def test_scan_beyond_32_bits_of_offset():
+    """The last sequences of a long batch, and the last steps of a long series (behind a step that forgets everything)."""
+    b, t, d = 70_000, 8, 4096
+    x, gate, dy = _long(b, t, d), _long(b, t, d), _long(b, t, d)
+    h0, dhl = rnd((b, d), torch.float32, 3), rnd((b, d), torch.float32, 5)
+    got, n = run_scan(x, gate, h0, None, dy, dhl), 3
+    scan_compare({k: v[-n:] for k, v in got.items()}, scan64(x[-n:], gate[-n:], h0[-n:], None, dy[-n:], dhl[-n:]))
+    del got
+    x, gate, dy = (v.view(1, -1, d)[:, :540_000] for v in (x, gate, dy))
+    assert x.numel() > 2 ** 31
+    n = 200
+    gate[:, -n] = -100.0
+    got = run_scan(x, gate, None, None, dy, dhl[-1:])
+    want = scan64(x[:, -n:], gate[:, -n:], None, None, dy[:, -n:], dhl[-1:])
+    for k in ("y", "dx", "dgate"):
+        check(k, got[k][:, 1 - n:], *(v[:, 1:] for v in want[k]))
+    check("h", got["h"], *want["h"])
