@@ -306,6 +306,21 @@ def test_linear_few_outputs_of_long_sums(m, n, k, dtype, act):
     linear_case(m, n, k, dtype, "none", bias=False, residual=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(4100, 2571, 2051), (4100, 2571, 2048), (4100, 2568, 2051), (2051, 4103, 2565)])
+def test_linear_large_and_ragged(m, n, k, dtype):
+    """Rows that are no whole 16-byte pieces, large enough to be laid out anew for the products."""
+    linear_case(m, n, k, dtype, "silu")
+    linear_case(m, n, k, dtype, "none", bias=False, residual=False)
+    x, w = rnd((m, k), dtype, 1).requires_grad_(), rnd((n, k), dtype, 2, k ** -0.5).requires_grad_()
+    from vae_amd import layers
+    dy = rnd((m, n), dtype, 5)
+    want = linear64(x.detach(), w.detach(), None, None, dy, "none")
+    for leaf, name in ((x, "dx"), (w, "dw")):  # one gradient at a time
+        got, = torch.autograd.grad(layers.linear(x, w), leaf, dy)
+        check(name, got, *want[name])
+
+
 def test_linear_strides():
     from vae_amd import layers
     for dtype in DTYPES:

@@ -101,6 +101,9 @@ struct GemmArgs {
     float slope;
     float* part;  // split sums: [slices][M][N] instead of c
     int kslice;
+    // What the large products may read of an operand: k (k contiguous) or rows (row contiguous) up to whole 16-byte pieces, where those lie
+    // in the operand's rows (zeros behind K; behind M and N it does not matter what)
+    int a_ext, b_ext;
 };
 
 template <typename T>
@@ -463,8 +466,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
     const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     Dma<T, BM, ARC, NT> da;
     Dma<T, BN, BRC, NT> db;
-    da.init((const T*)g.a, g.lda, m0, g.M, tid);
-    db.init((const T*)g.b, g.ldb, n0, g.N, tid);
+    da.init((const T*)g.a, g.lda, m0, ARC ? g.a_ext : g.M, tid);
+    db.init((const T*)g.b, g.ldb, n0, BRC ? g.b_ext : g.N, tid);
+    const int a_hi = ARC || k_hi < g.K ? k_hi : g.a_ext, b_hi = BRC || k_hi < g.K ? k_hi : g.b_ext;
     constexpr int DN = Dma<T, BM, ARC, NT>::N;
     static_assert(BM == BN, "one number of instructions for both operands");
     f32x4 acc[FM][FN];
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
         const int k = k_lo + h * HK<T>();
-        const i32x4 a = da.at(k, k_hi), b = db.at(k, k_hi);
+        const i32x4 a = da.at(k, a_hi), b = db.at(k, b_hi);
 #pragma unroll
         for (int j = 0; j < DN; ++j) da.issue(j, a, lbase + h * SLOT, da.kk >= k_hi - k), db.issue(j, b, lbase + h * SLOT + BM * HB, db.kk >= k_hi - k);
     }
@@ -487,7 +491,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
     for (int i = 0; i < FM; ++i) fa[0][i] = frag<T, BM, ARC, HB>(lds, wm + i * 16, 0, lane);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // slot 0 has been read
     uint32_t slot = 0;  // of the half tile in work
-    i32x4 a = da.at(k_lo + 4 * HK<T>(), k_hi), b = db.at(k_lo + 4 * HK<T>(), k_hi);  // of the half tile that is loaded next
+    i32x4 a = da.at(k_lo + 4 * HK<T>(), a_hi), b = db.at(k_lo + 4 * HK<T>(), b_hi);  // of the half tile that is loaded next
     bool tail = da.kk >= k_hi - (k_lo + 4 * HK<T>());
     for (int k0 = k_lo; k0 < k_hi; k0 += 2 * HK<T>()) {
 #pragma unroll
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmA
                 if (i == FM - 1) {  // (here the scalar unit is free; at a phase's head the matrix cores would wait for it)
                     int k5 = k0 + (5 + par) * HK<T>();
                     asm volatile("" : "+s"(k5));  // (nothing of it moves up)
-                    a = da.at(k5, k_hi), b = db.at(k5, k_hi);
+                    a = da.at(k5, a_hi), b = db.at(k5, b_hi);
                     tail = da.kk >= k_hi - k5;
                 }
             }
@@ -695,7 +699,7 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
         for (int64_t m = (int64_t)blockIdx.y * ACT_ROWS + r; m < M; m += (int64_t)gridDim.y * ACT_ROWS) {
             float v[8], p[8];
             load_part<T, 8>(v, dy + m * ldy + n, left, N >= 8);
-            if (auxk != AUX_NONE) {
+            if (auxk != AUX_NONE) {  // (what is loaded behind N is 0, and so is what comes of it)
                 const int64_t at = m * N + n;
                 if (auxk == AUX_U8) {
                     Pack<uint8_t, 8> q;
@@ -712,8 +716,8 @@ __global__ __launch_bounds__(256) void dense_dact_k(const T* dy, int64_t ldy, co
                     }
                     dense_act_grad8<sizeof(T) == 2>(v, p, act);
                 }
-                store_part<T, 8>(dp + m * ldp + n, v, left);
             }
+            if (dp != nullptr) store_part<T, 8>(dp + m * ldp + n, v, ldp - n);  // with the zeros behind N
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
@@ -754,11 +758,11 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
 
 // Can the operands go to LDS directly: rows that start and end on 16 bytes, a tile's rows within 31 bits of offset.
 template <typename T>
-bool whole_pieces(const GemmArgs& g, bool arc, bool brc) {
+bool whole_pieces(const GemmArgs& g) {
     constexpr int V = 16 / sizeof(T);
     const int64_t most = (int64_t)0x7fffffff / (256 * sizeof(T)) - 64;
-    return ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.lda % V == 0 && g.ldb % V == 0 && (arc ? g.M : g.K) % V == 0 &&
-           (brc ? g.N : g.K) % V == 0 && g.lda < most && g.ldb < most;
+    return ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.lda % V == 0 && g.ldb % V == 0 && g.a_ext % V == 0 && g.b_ext % V == 0 &&
+           g.lda < most && g.ldb < most;
 }
 
 // Tile and slices of k of a product: the pair that takes least by what was measured of each.  256 workgroups at a time, one a CU,
@@ -770,12 +774,12 @@ bool whole_pieces(const GemmArgs& g, bool arc, bool brc) {
 // 245 (128).  Split: 65 x 4,096 x 4,096 bf16 25 whole, 16 in slices; fp32 90, 45.
 struct GemmPlan {
     int tile, slices, kslice;
+    float us;
 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int es, bool whole) {
     constexpr float TILE_US[2][3][2] = {{{1.f, 0.30f}, {8.f, 0.457f}, {22.5f, 1.16f}}, {{1.5f, 0.58f}, {8.f, 2.f}, {0.f, 0.f}}};  // 16-bit, fp32: 64, 128, 256
     const int64_t bk = KB / es, kt = ceil_div64(K, bk);
     GemmPlan best = {};
-    float least = 0.f;
     for (int i = 0; i < (!whole ? 1 : es == 2 ? 3 : 2); ++i) {
         const int t = 64 << i;
         const int64_t tiles = ceil_div64(M, t) * ceil_div64(N, t);
@@ -793,15 +797,15 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int es, bool whole) {
             float us = (float)turns * (c[0] + (float)per * c[1]);
             if (turns == 1 && t < 256) us *= 1.15f;  // (a CU takes two of these tiles at once, and is better busy then)
             if (s > 1) us += 5.f + 2e-6f * (float)s * (float)M * (float)N;
-            if (best.tile == 0 || us < least) least = us, best = {t, (int)s, (int)(per * bk)};
+            if (best.tile == 0 || us < best.us) best = {t, (int)s, (int)(per * bk), us};
         }
     }
     if (best.slices == 1) best.kslice = (int)K;
     return best;
 }
 template <typename T>
-GemmPlan gemm_plan(const GemmArgs& g, bool arc, bool brc) {
-    return gemm_plan(g.M, g.N, g.K, sizeof(T), whole_pieces<T>(g, arc, brc));
+GemmPlan gemm_plan(const GemmArgs& g) {
+    return gemm_plan(g.M, g.N, g.K, sizeof(T), whole_pieces<T>(g));
 }
 // floats that the slices take at most, wherever the operands lie
 int64_t gemm_split_floats(int64_t M, int64_t N, int64_t K, int es) {
@@ -820,6 +824,46 @@ int gemm(GemmArgs g, const GemmPlan& p, hipStream_t s) {
     return gemm_inst<T, 128, ARC, BRC>(g, p.slices, s);
 }
 
+// Operands whose rows are not whole pieces, copied into rows that are, zeros behind their end.  16-bit types only: fp32 tiles of 64 come
+// within 5 % of the larger ones.  A copy is read and written at about 4.5 TB/s and its launch takes 4 us; it is made where the larger tiles
+// bring in more than that (4,095 x 4,097 x 4,093 bf16 forward: 336 us in tiles of 64, 195 with the copies; 2,047 x 2,049 x 2,051, left in those: 55).
+constexpr float PAD_US = 4.f, PAD_US_A_BYTE = 2.f / 4.5e6f;
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+bool forward_pads(int64_t M, int64_t N, int64_t K, int es) {
+    if (es != 2 || K % 8 == 0) return false;
+    return gemm_plan(M, N, K, es, true).us + PAD_US + PAD_US_A_BYTE * (float)es * (float)K * (float)(M + N) < gemm_plan(M, N, K, es, false).us;
+}
+bool backward_pads(int64_t M, int64_t N, int64_t K, int es, int act) {
+    if (es != 2 || (K % 8 == 0 && N % 8 == 0)) return false;
+    float us = gemm_plan(M, K, N, es, true).us + gemm_plan(N, K, M, es, true).us;
+    if (K % 8 != 0) us += PAD_US + PAD_US_A_BYTE * (float)es * (float)K * (float)(M + N);
+    if (N % 8 != 0 && act == VAE_ACT_NONE) us += PAD_US + PAD_US_A_BYTE * (float)es * (float)N * (float)M;
+    return us < gemm_plan(M, K, N, es, false).us + gemm_plan(N, K, M, es, false).us;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void dense_pad_k(const T* a, int64_t lda, int64_t rows_a, T* pa, const T* b, int64_t ldb, int64_t rows_b, T* pb, int cols) {
+    const int per = (cols + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / per;
+    if (m >= rows_a + rows_b) return;
+    const int c = (int)(i - m * per) * 8;
+    Pack<T, 8> r;
+    load_raw<T, 8>(r, (m < rows_a ? a + m * lda : b + (m - rows_a) * ldb) + c, cols - c, cols >= 8);
+    *reinterpret_cast<uint4*>((m < rows_a ? pa + m * per * 8 : pb + (m - rows_a) * per * 8) + c) = __builtin_bit_cast(uint4, r);
+}
+// a and b (null: not wanted) to pa and pb, their strides and pointers changed
+template <typename T>
+int dense_pad(const T*& a, int64_t& lda, int64_t rows_a, T* pa, const T*& b, int64_t& ldb, int64_t rows_b, T* pb, int cols, hipStream_t s) {
+    if (a == nullptr) rows_a = 0;
+    if (b == nullptr) rows_b = 0;
+    const int64_t blocks = ceil_div64((rows_a + rows_b) * (pad8(cols) / 8), 256);
+    if (blocks > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "dense: %lld blocks", (long long)blocks);
+    dense_pad_k<T><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a, lda, rows_a, pa, b, ldb, rows_b, pb, cols);
+    VAE_LAUNCH_CHECK("dense_pad_k");
+    if (a != nullptr) a = pa, lda = pad8(cols);
+    if (b != nullptr) b = pb, ldb = pad8(cols);
+    return VAE_OK;
+}
+
 // Slices of the rows: about 2048 workgroups in all, 256 at most (rows of partial sums)
 constexpr int DACT_MAX = 256;
 int dact_rows(int64_t M, int64_t N) {
@@ -833,24 +877,41 @@ int dact_rows(int64_t M, int64_t N) {
 int64_t dp_stride(int64_t N, int es) { return ceil_div64(N, 16 / es) * (16 / es); }
 
 struct DenseWs {  // workspace of the backward pass, in floats
-    int64_t dp, split_w, split_x, cols, total;
+    int64_t dp, split_w, split_x, cols, pad_w, pad_x, total;
+    bool keeps_dp, pads;  // is dp written, are w and x copied
 };
 DenseWs dense_ws(int64_t M, int64_t N, int64_t K, int dtype, int act) {
     DenseWs l;
     const int es = vae_type_size(dtype);
     const int64_t a = 64;
+    const bool pads = backward_pads(M, N, K, es, act);
+    l.keeps_dp = act != VAE_ACT_NONE || (pads && N % 8 != 0);
+    l.pads = pads && K % 8 != 0;
     l.dp = 0;
-    l.split_w = l.dp + (act == VAE_ACT_NONE ? 0 : ceil_div64(ceil_div64(M * dp_stride(N, es) * es, 4), a) * a);
+    l.split_w = l.dp + (l.keeps_dp ? ceil_div64(ceil_div64(M * dp_stride(N, es) * es, 4), a) * a : 0);
     l.split_x = l.split_w + ceil_div64(gemm_split_floats(N, K, M, es), a) * a;
     l.cols = l.split_x + ceil_div64(gemm_split_floats(M, K, N, es), a) * a;
-    l.total = l.cols + dact_rows(M, N) * N;
+    l.pad_w = l.cols + ceil_div64(dact_rows(M, N) * N, a) * a;
+    l.pad_x = l.pad_w + (l.pads ? ceil_div64(N * pad8(K) / 2, a) * a : 0);
+    l.total = l.pad_x + (l.pads ? M * pad8(K) / 2 : 0);
     return l;
 }
 
+int64_t forward_split(int64_t M, int64_t N, int64_t K, int es) { return ceil_div64(gemm_split_floats(M, N, K, es), 64) * 64; }
 template <typename T>
 int dense_forward_t(GemmArgs& g, float* workspace, hipStream_t s) {
     if (dense_few(g.M, g.K, sizeof(T))) return dense_rows<T>(g, s);
-    const GemmPlan p = gemm_plan<T>(g, false, false);
+    g.a_ext = g.b_ext = g.K;
+    if constexpr (sizeof(T) == 2) {
+        if (forward_pads(g.M, g.N, g.K, 2)) {
+            if (workspace == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null workspace");
+            T* pa = (T*)(workspace + forward_split(g.M, g.N, g.K, 2));
+            const T *a = (const T*)g.a, *b = (const T*)g.b;
+            if (int rc = dense_pad<T>(a, g.lda, g.M, pa, b, g.ldb, g.N, pa + (int64_t)g.M * pad8(g.K), g.K, s)) return rc;
+            g.a = a, g.b = b, g.a_ext = g.b_ext = (int)pad8(g.K);
+        }
+    }
+    const GemmPlan p = gemm_plan<T>(g);
     if (p.slices > 1) {
         if (workspace == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null workspace");
         g.part = workspace;
@@ -870,17 +931,28 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
     const int auxk = aux_kind(act, dtype), ny = dact_rows(M, N);
     const T* dp = dy;
     int64_t lddp = lddy;
-    if (auxk != AUX_NONE || db != nullptr) {
-        T* out = (T*)(ws + lay.dp);
+    if (lay.keeps_dp || db != nullptr) {
+        T* out = lay.keeps_dp ? (T*)(ws + lay.dp) : nullptr;
         dense_dact_k<T><<<dim3((unsigned)ceil_div64(N, 256), ny), dim3(256), 0, s>>>(dy, lddy, aux, out, dp_stride(N, sizeof(T)),
                                                                                    db != nullptr ? ws + lay.cols : nullptr, M, N, act, auxk, slope);
         VAE_LAUNCH_CHECK("dense_dact_k");
-        if (auxk != AUX_NONE) dp = out, lddp = dp_stride(N, sizeof(T));
+        if (lay.keeps_dp) dp = out, lddp = dp_stride(N, sizeof(T));
+    }
+    const int n_ext = lay.keeps_dp ? (int)dp_stride(N, sizeof(T)) : N;
+    int k_ext = K;
+    if constexpr (sizeof(T) == 2) {
+        if (lay.pads) {
+            if (dx == nullptr) w = nullptr;
+            if (dw == nullptr) x = nullptr;
+            if (w != nullptr || x != nullptr)
+                if (int rc = dense_pad<T>(w, ldw, N, (T*)(ws + lay.pad_w), x, ldx, M, (T*)(ws + lay.pad_x), K, s)) return rc;
+            k_ext = (int)pad8(K);
+        }
     }
     GemmArgs gx = {}, gw = {};
-    gx.a = dp, gx.lda = lddp, gx.b = w, gx.ldb = ldw, gx.c = dx, gx.ldc = K, gx.M = M, gx.N = K, gx.K = N;
-    gw.a = dp, gw.lda = lddp, gw.b = x, gw.ldb = ldx, gw.c = dw, gw.ldc = K, gw.M = N, gw.N = K, gw.K = M;
-    const GemmPlan pw = gemm_plan<T>(gw, true, true), px = gemm_plan<T>(gx, false, true);
+    gx.a = dp, gx.lda = lddp, gx.b = w, gx.ldb = ldw, gx.c = dx, gx.ldc = K, gx.M = M, gx.N = K, gx.K = N, gx.a_ext = n_ext, gx.b_ext = k_ext;
+    gw.a = dp, gw.lda = lddp, gw.b = x, gw.ldb = ldx, gw.c = dw, gw.ldc = K, gw.M = N, gw.N = K, gw.K = M, gw.a_ext = n_ext, gw.b_ext = k_ext;
+    const GemmPlan pw = gemm_plan<T>(gw), px = gemm_plan<T>(gx);
     Slices<T> jw = {ws + lay.split_w, (int64_t)N * K, dw, pw.slices, 0}, jx = {ws + lay.split_x, (int64_t)M * K, dx, px.slices, 0};
     if (dw != nullptr && jw.slices > 1) gw.part = ws + lay.split_w, jw.blocks = (int)ceil_div64(jw.n, 1024);
     if (dx != nullptr && jx.slices > 1) gx.part = ws + lay.split_x, jx.blocks = (int)ceil_div64(jx.n, 1024);
@@ -936,7 +1008,8 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
 
 extern "C" int64_t vae_dense_forward_workspace_floats(int64_t M, int64_t N, int64_t K, int dtype) {
     if (M < 1 || N < 1 || K < 1 || vae_type_size(dtype) == 0 || dense_few(M, K, vae_type_size(dtype))) return 0;
-    return gemm_split_floats(M, N, K, vae_type_size(dtype));
+    const int es = vae_type_size(dtype);
+    return forward_split(M, N, K, es) + (forward_pads(M, N, K, es) ? (M + N) * pad8(K) / 2 : 0);
 }
 
 extern "C" int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype) {
