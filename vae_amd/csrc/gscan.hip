@@ -427,13 +427,16 @@ __global__ __launch_bounds__(64) void gscan_step_k(const GsArgs a) {
 
 int64_t gs_columns(int B, int D, int V) { return ceil_div64((int64_t)B * ((D + V - 1) / V), 64); }
 
-// What a launch looks like.  V features a lane: as many as leave 256 columns of workgroups, at most 8 bytes forward and 8 and 4 bytes
-// (fp32 and 16-bit types) backward, where more would not stay in registers; never more than D, and four only where a row holds whole fours
-// (1,000 x 1,000 x 67 bf16: 140 us, 173 with fours across the rows' ends).
+// What a launch looks like.  V features a lane: as many as leave 256 columns of workgroups, and never more than D; two at most (four
+// forward for a few 16-bit steps), as four are no faster (8 x 1,024 x 16,384 bf16 forward: 153 us both) and the backward pass has no
+// registers for them.  For a long series one where two make 257 to 384 columns, which 256 CUs take in two turns and twice as many of half
+// the size in one and a half: 8 x 1,024 x 4,800 fp32 100 us forward and 171 backward, with two a lane 116 and 197; 8 x 1,024 x 4,096 (256
+// columns) 89 and 150, with two 82 and 130.  (513 to 640 columns: better in whole rows, 183 and 170 for 8 x 1,024 x 8,320, worse in ragged
+// ones, 430 and 481 for the backward pass of 1,000 x 1,000 x 67.)
 //   W waves a workgroup: as few as hold a short series, or (forward; the backward pass starts from states 64 steps apart) most of its
 // last tile: 4,096 x 9 x 1,800 fp32 162 us with two, 250 with four; 1,024 x 65 x 1,000 bf16 100 with four, 154 with eight.  16 for a long
 // series while each column of channels has a CU of its own, 8 beyond: 8 x 1,024 x 2,304 bf16 31 us forward and 58 backward, 36 and 64 with
-// 16 (four for V of 2 and 4 would cost up to a fifth of the backward pass).
+// 16 (four for V = 2 would cost up to a fifth of the backward pass).
 //   Parts of the time axis: as many as make 512 workgroups.  They read x and gate (backward: gate and dy) twice, but let more workgroups
 // at them than the channels make.  In parts and in one go, T = 4,096: fp32 forward 31 and 62 us at 24 columns, 60 and 62 at 64, 70 and 63
 // at 72 (T = 16,384: 266 and 307 at 64, 331 and 333 at 80), backward 161 and 164 at 104, 191 and 181 at 128; bf16 forward 43 and 61 at
@@ -444,9 +447,9 @@ struct GsPlan {
 };
 GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
     GsPlan p;
-    p.V = esize == 2 && fwd ? 4 : 2;
-    if (p.V == 4 && D % 4 != 0) p.V = 2;
+    p.V = esize == 2 && fwd && T <= GS_S ? 4 : 2;
     while (p.V > 1 && (p.V > D || gs_columns(B, D, p.V) < 256)) p.V >>= 1;
+    if (p.V == 2 && T > GS_TILE && gs_columns(B, D, 2) > 256 && gs_columns(B, D, 2) <= 384) p.V = 1;
     const int64_t cols = gs_columns(B, D, p.V);
     if (T <= GS_S) p.W = 1;
     else if (T <= 2 * GS_S) p.W = 2;
@@ -496,7 +499,7 @@ int gs_run(GsArgs& a) {
     VAE_GS(1)
     VAE_GS(2)
     if constexpr (sizeof(T) == 2 && FWD) {
-        VAE_GS(4)
+        if (p.V == 4) return gs_launch<T, 4, 1, FWD>(a);
     }
 #undef VAE_GS
     VAE_FAIL(VAE_EINVAL, "gated_scan: no launch for V = %d, W = %d", p.V, p.W);
