@@ -625,7 +625,7 @@ struct Slices {
 };
 template <typename T>
 __global__ __launch_bounds__(256) void dense_join_k(const Slices<T> dw, const Slices<T> dx, const float* cols, int rows, int N, T* db) {
-    const int b = (int)blockIdx.x - dw.blocks, join_blocks = dw.blocks + dx.blocks;
+    const int b = (int)blockIdx.x - dw.blocks;
     if (b < dx.blocks) {
         const Slices<T>& j = b < 0 ? dw : dx;
         const int64_t i = ((int64_t)(b < 0 ? (int)blockIdx.x : b) * 256 + threadIdx.x) * 4;
@@ -640,16 +640,16 @@ __global__ __launch_bounds__(256) void dense_join_k(const Slices<T> dw, const Sl
         store_part<T, 4>(j.out + i, s, j.n - i);
         return;
     }
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = ((int)blockIdx.x - join_blocks) * 64 + lane;
-    float s = 0.f;
+    __shared__ double red[4][64];  // (64 bits: as in part_cols_k)
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = (b - dx.blocks) * 64 + lane;
+    double s = 0.;
     if (col < N) {
 #pragma unroll 8
-        for (int r = w; r < rows; r += 4) s += cols[(int64_t)r * N + col];
+        for (int r = w; r < rows; r += 4) s += (double)cols[(int64_t)r * N + col];
     }
     red[w][lane] = s;
     __syncthreads();
-    if (w == 0 && col < N) db[col] = (T)(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
+    if (w == 0 && col < N) db[col] = (T)(float)(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
 }
 
 // ... and the forward pass: a lane adds 8 neighbouring values and gives them the epilogue that a whole product has in store_tile.

@@ -108,27 +108,28 @@ __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
     }
 }
 
-// Column sums of `rows` rows of n partial sums, in a fixed order: 64 columns a workgroup, 16 waves that take every 16th row.
+// Column sums of `rows` rows of n partial sums, in a fixed order: 64 columns a workgroup, 16 waves that take every 16th row.  In
+// 64 bits: a chain of 64 additions in 32 would cost more than all that the partial sums have lost, and memory is what it waits for.
 // Column c goes to out0[c], or to out1[c - split] from `split` on; a null output is skipped.
 template <typename T>
 __global__ __launch_bounds__(1024) void part_cols_k(const float* part, int rows, int64_t n, T* out0, T* out1, int64_t split) {
-    __shared__ float red[16][64];
+    __shared__ double red[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-    float s = 0.f;
+    double s = 0.;
     if (c < n) {
 #pragma unroll 8
-        for (int r = w; r < rows; r += 16) s += part[r * n + c];
+        for (int r = w; r < rows; r += 16) s += (double)part[r * n + c];
     }
     red[w][lane] = s;
     __syncthreads();
     if (w != 0 || c >= n) return;
-    s = 0.f;
+    s = 0.;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += red[i][lane];
     if (c < split) {
-        if (out0 != nullptr) out0[c] = (T)s;
+        if (out0 != nullptr) out0[c] = (T)(float)s;
     } else if (out1 != nullptr) {
-        out1[c - split] = (T)s;
+        out1[c - split] = (T)(float)s;
     }
 }
