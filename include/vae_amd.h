@@ -343,7 +343,7 @@ int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
 
 /* Linear layer p = x w^T + bias, y = act(p) + res: x M x K, w N x K, res and y M x N; bias (N), res optional.  act = VAE_ACT_*
  * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.  workspace
- * (vae_dense_forward_workspace_floats; NULL where that is 0): sums of products of few outputs, which are split over k.
+ * (vae_dense_forward_workspace_floats; NULL where that is 0): slices of products of few outputs, copies of large ragged operands.
  * Backward: dp = dy act'(p); dx = dp w (M x K, dense), dw = dp^T x (N x K, dense), db = column sums of dp; each optional.  The
  * residual's gradient is dy itself. */
 int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype);

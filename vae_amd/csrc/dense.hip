@@ -309,10 +309,10 @@ __device__ __forceinline__ void tile_of(int tile, int M, int N, int BM, int BN, 
     m = grp * 8 + (in - n * h);
 }
 
-// C tile of 64 x 64 by four waves, for products too small for the kernel below and for operands of any alignment.  The tiles of
-// the operands pass registers, AHEAD of them in flight: with a workgroup or two a CU a tile's loads take longer than its products,
-// and only loads in flight hide that (256 x 4,096 x 4,096 bf16 forward: 46 us with one tile ahead, 29 with four).  The matrix instruction's first operand is B: a lane then
-// holds four neighbouring columns n of one row m of C.
+// C tile of 64 x 64 by four waves, for products too small for the kernel below and for operands of any alignment.  The tiles of the
+// operands pass registers, AHEAD of them in flight: with a workgroup or two a CU a tile's loads take longer than its products, and
+// only loads in flight hide that (256 x 4,096 x 4,096 bf16 forward: 46 us with one tile ahead, 29 with four).  The matrix
+// instruction's first operand is B: a lane then holds four neighbouring columns n of one row m of C.
 template <typename T, bool ARC, bool BRC>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tile, int slice, char* lds) {
     constexpr int BM = 64, BN = 64, WM = 2, WN = 2, AHEAD = 4, NT = WM * WN * 64, V = 16 / sizeof(T), FM = BM / WM / 16, FN = BN / WN / 16;

@@ -4,7 +4,7 @@
 // the sum of (x - mean)^2 of the same registers: two passes over the values, one over memory.
 //   y  = (x - mean) rstd w + b
 //   g  = dy w,  dx = rstd (g - mean(g) - xhat mean(g xhat)),  dw = sum over rows of dy xhat,  db = sum over rows of dy
-// Bound: bytes.  Groups of 8..64 lanes (several rows a wave) keep the lanes of short rows busy and sum with lane shuffles
+// Bound: bytes.  Groups of 4..64 lanes (several rows a wave) keep the lanes of short rows busy and sum with lane shuffles
 // alone; longer rows take a workgroup.  The backward pass keeps dw and db of the lane's own columns in registers over all rows
 // that its group visits; workgroups leave one row of partials each, which a second launch adds in a fixed order (no atomics:
 // two runs give the same bits).

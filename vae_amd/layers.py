@@ -2,11 +2,12 @@
 
 They stand next to the BatchNorm, Linear and Conv1d ops of the model programs for modules that treat every time step of a
 window as a row: a module built from them trains through `vae_amd.train.train` (autograd path) with `vae_amd.optim.Adam`.
-Each is one or two launches forward and differentiable once.  Tensors are fp32, bf16 or fp16 on an MI355X; sums, statistics and
-states are fp32 (include/vae_amd.h, vae_layer_norm_* / vae_dense_* / vae_gated_scan_*).  Calls run on the current stream of the
-tensors' device, allocate through torch's allocator and can be captured in a graph.  Before a backward pass is captured, drop the
-eager graphs (losses, outputs) of the same leaves: torch ties a leaf's gradient node to the stream of the first graph that it was in
-and would wait for that stream inside the capture, which ends the process.
+Each is one launch forward, or two or three where sums are split or ragged rows laid out anew, and differentiable once.
+Tensors are fp32, bf16 or fp16 on an MI355X; sums, statistics and states are fp32 (include/vae_amd.h, vae_layer_norm_* /
+vae_dense_* / vae_gated_scan_*).  Calls run on the current stream of the tensors' device, allocate through torch's allocator
+and can be captured in a graph.  Before a backward pass is captured, drop the eager graphs (losses, outputs) of the same
+leaves: torch ties a leaf's gradient node to the stream of the first graph that it was in and would wait for that stream inside
+the capture, which ends the process.
 """
 import torch
 from torch.autograd.function import once_differentiable
