@@ -72,6 +72,15 @@ def _rows(t, cols):
     return t.contiguous(), rows, cols
 
 
+def _once(backward):
+    """once_differentiable, at the price of one question where no second derivative is asked for (2 of 109 us a pass otherwise)."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _needs_grad(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -103,7 +112,7 @@ class _NormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         xr, weight, bias, stat = ctx.saved_tensors
         rows, C, ldx, device, code, wtype = ctx.geom
@@ -173,7 +182,7 @@ class _LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         xr, wr, aux = ctx.saved_tensors
         M, N, K, ldx, ldw, act, slope, device, code = ctx.geom
@@ -252,7 +261,7 @@ class _ScanFn(torch.autograd.Function):
         return y, hl
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dhl):
         xs, gs, h0, lengths, kept = ctx.saved_tensors
         B, T, D = xs.shape
