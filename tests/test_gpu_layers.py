@@ -372,6 +372,23 @@ def test_linear_far_values_and_nan_rows():
         assert torch.equal(y[keep], clean[keep])
 
 
+@pytest.mark.parametrize("view", [lambda t: t[:, -1:], lambda t: t[:, -1], lambda t: t[:, 2:5], lambda t: t[:, ::3], lambda t: t[1:2, 3:4], lambda t: t[:, :, :40],
+                                  lambda t: t[:, None, 1], lambda t: t.transpose(0, 1), lambda t: t[..., ::2], lambda t: t[:1].expand(5, -1, -1)])
+def test_views_of_windows_equal_their_copies(view):
+    """Steps taken out of windows go in as they lie; values and gradients are those of a copy."""
+    from vae_amd import layers
+    base = rnd((6, 11, 48), torch.bfloat16, 1)
+    x = view(base)
+    w, nw = rnd((24, x.shape[-1]), torch.bfloat16, 2), rnd(x.shape[-1], torch.float32, 3)
+    res = []
+    for t in (x, x.clone(memory_format=torch.contiguous_format)):
+        t = t.detach().requires_grad_()
+        y, z = layers.linear(t, w, act="silu"), layers.layer_norm(t, nw)
+        res.append([y.detach(), z.detach(), *torch.autograd.grad(y, t, torch.ones_like(y)), *torch.autograd.grad(z, t, view(rnd(base.shape, torch.bfloat16, 4)))])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
 def test_linear_one_row_of_any_stride():
     """Through the C entry: the strides of a single row say nothing, 0 among them.  Products of two bf16 values are exact in fp32, so
     dW is its own rounding; dx: a sum of n terms."""

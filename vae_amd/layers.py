@@ -64,11 +64,19 @@ def _rows(t, cols):
     rows = t.numel() // cols
     if t.is_contiguous():
         return t, rows, cols
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
-        return t, rows, t.stride(0)
-    if t.dim() > 2 and t.stride(-1) == 1 and t.stride(-2) >= cols and all(
-            t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2)):
-        return t, rows, t.stride(-2)
+    if t.stride(-1) == 1:
+        ld, n = 0, 1
+        for size, stride in zip(t.shape[-2::-1], t.stride()[-2::-1]):
+            if size == 1:  # (the last step of every window, say)
+                continue
+            if n == 1:
+                ld = stride
+            elif stride != ld * n:
+                ld = 0
+                break
+            n *= size
+        if ld >= cols:
+            return t, rows, ld
     return t.contiguous(), rows, cols
 
 
