@@ -329,17 +329,18 @@ int vae_window_gather(const float* series, int C, int64_t T, int L, const int64_
  * dtype = VAE_T_* of the tensors; strides are in elements, rows are contiguous (any alignment, any stride >= the row).  All
  * sums, statistics and states are fp32.  Workspaces are caller-owned, sized by the *_floats / *_bytes queries (host-only), need no
  * clearing and hold nothing between calls; calls that may overlap need a workspace each.  Results are bit-identical from run to
- * run (no float atomics).
+ * run (no float atomics).  Sizes are 64-bit so that what is too large is seen and refused: rows and columns of a norm up to 2^31 - 1,
+ * M, N, K of a linear layer up to 2^30 - 1, T up to 2^31 - 2^16, B D up to 2^31 - 1, and no launch of 2^32 threads.
  *
  * Layer norm over rows of C: y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) with the biased variance.  w, b: type wtype
  * (VAE_T_F32 or dtype), NULL = 1 / 0.  mean, rstd (rows floats each; both or neither): what the backward pass needs.
  * Backward: dx, dw, db are optional each; dw and db are the sums over all rows, in wtype; workspace only for those. */
 int vae_layer_norm_forward(const void* x, int64_t ldx, const void* w, const void* b, void* y, int64_t ldy, float* mean,
-                           float* rstd, int64_t rows, int C, float eps, int dtype, int wtype, vae_stream_t stream);
-int64_t vae_layer_norm_workspace_floats(int64_t rows, int C);
+                           float* rstd, int64_t rows, int64_t C, float eps, int dtype, int wtype, vae_stream_t stream);
+int64_t vae_layer_norm_workspace_floats(int64_t rows, int64_t C);
 int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
-                            const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* workspace, int64_t rows, int C,
-                            int dtype, int wtype, vae_stream_t stream);
+                            const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* workspace, int64_t rows,
+                            int64_t C, int dtype, int wtype, vae_stream_t stream);
 
 /* Linear layer p = x w^T + bias, y = act(p) + res: x M x K, w N x K, res and y M x N; bias (N), res optional.  act = VAE_ACT_*
  * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.  workspace
@@ -348,12 +349,12 @@ int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * residual's gradient is dy itself. */
 int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype);
 int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
-                      void* y, int64_t ldy, void* aux, float* workspace, int M, int N, int K, int act, float slope, int dtype,
-                      vae_stream_t stream);
+                      void* y, int64_t ldy, void* aux, float* workspace, int64_t M, int64_t N, int64_t K, int act, float slope,
+                      int dtype, vae_stream_t stream);
 int64_t vae_dense_forward_workspace_floats(int64_t M, int64_t N, int64_t K, int dtype);
 int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype);
 int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* aux,
-                       void* dx, void* dw, void* db, float* workspace, int M, int N, int K, int act, float slope, int dtype,
+                       void* dx, void* dw, void* db, float* workspace, int64_t M, int64_t N, int64_t K, int act, float slope, int dtype,
                        vae_stream_t stream);
 
 /* Gated linear recurrence over B sequences of T steps of D features: f = sigmoid(gate), h_t = f h_{t-1} + (1 - f) x_t, y_t = h_t.
@@ -361,15 +362,15 @@ int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * optional (absent: zeros).  lengths (B, optional, clamped to 0..T): steps at and behind a sequence's length hold the state, whatever
  * x, gate and dy contain there; y, dx and dgate are 0 there; h_last is the state behind the last step that counts.
  * kept (vae_gated_scan_kept_floats; NULL when no backward pass follows): states that the backward pass starts its tiles from. */
-int64_t vae_gated_scan_kept_floats(int B, int T, int D);
-int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype);
+int64_t vae_gated_scan_kept_floats(int64_t B, int64_t T, int64_t D);
+int64_t vae_gated_scan_workspace_floats(int64_t B, int64_t T, int64_t D, int dtype);
 int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st,
-                           const float* h0, const int32_t* lengths, void* y, float* h_last, float* kept, float* workspace, int B,
-                           int T, int D, int dtype, vae_stream_t stream);
+                           const float* h0, const int32_t* lengths, void* y, float* h_last, float* kept, float* workspace,
+                           int64_t B, int64_t T, int64_t D, int dtype, vae_stream_t stream);
 int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last, const void* x, int64_t x_sb,
                             int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st, const float* h0, const int32_t* lengths,
-                            const float* kept, void* dx, void* dgate, float* dh0, float* workspace, int B, int T, int D, int dtype,
-                            vae_stream_t stream);
+                            const float* kept, void* dx, void* dgate, float* dh0, float* workspace, int64_t B, int64_t T, int64_t D,
+                            int dtype, vae_stream_t stream);
 
 /* hipGraph capture of an arbitrary sequence of the calls above: begin, issue calls on the
  * returned stream, end -> handle; launch replays on `stream`. */

@@ -98,18 +98,18 @@ def lib():
     L.vae_adam_step_hyper.argtypes = [vp, vp, vp, vp, i64, vp, vp, vp]
     L.vae_randn.argtypes = [vp, i64, vp, vp]
     L.vae_window_gather.argtypes = [vp, i32, i64, i32, vp, i32, vp, vp]
-    L.vae_layer_norm_forward.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, f32, i32, i32, vp]
-    L.vae_layer_norm_workspace_floats.argtypes = [i64, i32]
-    L.vae_layer_norm_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
+    L.vae_layer_norm_forward.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, i64, f32, i32, i32, vp]
+    L.vae_layer_norm_workspace_floats.argtypes = [i64, i64]
+    L.vae_layer_norm_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i64, i32, i32, vp]
     L.vae_dense_aux_bytes.argtypes = [i64, i64, i32, i32]
-    L.vae_dense_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, f32, i32, vp]
+    L.vae_dense_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, i64, i64, i64, i32, f32, i32, vp]
     L.vae_dense_forward_workspace_floats.argtypes = [i64, i64, i64, i32]
     L.vae_dense_workspace_floats.argtypes = [i64, i64, i64, i32, i32]
-    L.vae_dense_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, i32, vp]
-    L.vae_gated_scan_kept_floats.argtypes = [i32, i32, i32]
-    L.vae_gated_scan_workspace_floats.argtypes = [i32, i32, i32, i32]
-    L.vae_gated_scan_forward.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
-    L.vae_gated_scan_backward.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]
+    L.vae_dense_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i32, f32, i32, vp]
+    L.vae_gated_scan_kept_floats.argtypes = [i64, i64, i64]
+    L.vae_gated_scan_workspace_floats.argtypes = [i64, i64, i64, i32]
+    L.vae_gated_scan_forward.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]
+    L.vae_gated_scan_backward.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, vp]
     for name in ("vae_layer_norm_workspace_floats", "vae_dense_aux_bytes", "vae_dense_forward_workspace_floats",
                  "vae_dense_workspace_floats", "vae_gated_scan_kept_floats", "vae_gated_scan_workspace_floats"):
         getattr(L, name).restype = i64

@@ -737,6 +737,8 @@ template <typename T, int B, bool ARC, bool BRC>
 int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
     constexpr int bytes = 4 * B * KB;
     static_assert(4 * 32 * (B / 2 + 4) * 4 <= bytes, "the epilogue's LDS");
+    const int64_t tiles = ceil_div64(g.N, B) * ceil_div64(g.M, B);
+    VAE_FITS("gemm_k", tiles, 256);
     void (*k)(const GemmArgs);
     if constexpr (B == 64) k = gemm_k<T, ARC, BRC>;
     else k = gemm_dma_k<T, B, B, ARC, BRC>;
@@ -749,8 +751,6 @@ int gemm_inst(const GemmArgs& g, int slices, hipStream_t s) {
             if (dev < 64) granted.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
         }
     }
-    const int64_t tiles = ceil_div64(g.N, B) * ceil_div64(g.M, B);
-    if (tiles > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "gemm: %lld tiles", (long long)tiles);
     k<<<dim3((unsigned)tiles, 1, slices), dim3(256), bytes, s>>>(g);
     VAE_LAUNCH_CHECK("gemm_k");
     return VAE_OK;
@@ -856,7 +856,7 @@ int dense_pad(const T*& a, int64_t& lda, int64_t rows_a, T* pa, const T*& b, int
     if (a == nullptr) rows_a = 0;
     if (b == nullptr) rows_b = 0;
     const int64_t blocks = ceil_div64((rows_a + rows_b) * (pad8(cols) / 8), 256);
-    if (blocks > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "dense: %lld blocks", (long long)blocks);
+    VAE_FITS("dense_pad_k", blocks, 256);
     dense_pad_k<T><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a, lda, rows_a, pa, b, ldb, rows_b, pb, cols);
     VAE_LAUNCH_CHECK("dense_pad_k");
     if (a != nullptr) a = pa, lda = pad8(cols);
@@ -957,7 +957,9 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
     if (dw != nullptr && jw.slices > 1) gw.part = ws + lay.split_w, jw.blocks = (int)ceil_div64(jw.n, 1024);
     if (dx != nullptr && jx.slices > 1) gx.part = ws + lay.split_x, jx.blocks = (int)ceil_div64(jx.n, 1024);
     if (dx != nullptr && dw != nullptr && pw.tile == 64 && px.tile == 64) {
-        const int tw = (int)(ceil_div64(N, 64) * ceil_div64(K, 64)), tx = (int)(ceil_div64(M, 64) * ceil_div64(K, 64));
+        const int64_t lw = ceil_div64(N, 64) * ceil_div64(K, 64), lx = ceil_div64(M, 64) * ceil_div64(K, 64);
+        VAE_FITS("gemm_pair_k", lw * jw.slices + lx * jx.slices, 256);
+        const int tw = (int)lw, tx = (int)lx;
         gw.kslice = pw.kslice, gx.kslice = px.kslice;
         gemm_pair_k<T><<<dim3((unsigned)(tw * jw.slices + tx * jx.slices)), dim3(256), 2 * 128 * KB, s>>>(gw, tw, tw * jw.slices, gx, tx);
         VAE_LAUNCH_CHECK("gemm_pair_k");
@@ -975,10 +977,11 @@ int dense_backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T
     return VAE_OK;
 }
 
+constexpr int64_t DENSE_MOST = 0x3fffffff;
 int dense_check(const char* what, int64_t M, int64_t N, int64_t K, int act, int dtype) {
     if (vae_type_size(dtype) == 0) VAE_FAIL(VAE_EINVAL, "%s: type %d (f32, bf16 or f16)", what, dtype);
     if (act < VAE_ACT_NONE || act > VAE_ACT_SILU) VAE_FAIL(VAE_EINVAL, "%s: activation %d", what, act);
-    if (M < 0 || N < 1 || K < 1 || M > 0x3fffffff || N > 0x3fffffff || K > 0x3fffffff)
+    if (M < 0 || N < 1 || K < 1 || M > DENSE_MOST || N > DENSE_MOST || K > DENSE_MOST)
         VAE_FAIL(VAE_EINVAL, "%s: M = %lld, N = %lld, K = %lld", what, (long long)M, (long long)N, (long long)K);
     return VAE_OK;
 }
@@ -990,8 +993,8 @@ extern "C" int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype)
 }
 
 extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
-                                 void* y, int64_t ldy, void* aux, float* workspace, int M, int N, int K, int act, float slope, int dtype,
-                                 vae_stream_t stream) {
+                                 void* y, int64_t ldy, void* aux, float* workspace, int64_t M, int64_t N, int64_t K, int act, float slope,
+                                 int dtype, vae_stream_t stream) {
     if (int rc = dense_check("dense_forward", M, N, K, act, dtype)) return rc;
     if (M == 0) return VAE_OK;
     if (x == nullptr || w == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "dense_forward: null buffer");
@@ -999,7 +1002,7 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
     if (N == 1) ldw = K;  // (a single row's stride may be anything)
     GemmArgs g = {};
     g.a = x, g.lda = ldx, g.b = w, g.ldb = ldw, g.c = y, g.ldc = ldy, g.bias = bias, g.res = res, g.ldr = ldr;
-    g.M = M, g.N = N, g.K = K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
+    g.M = (int)M, g.N = (int)N, g.K = (int)K, g.act = act, g.slope = slope, g.auxk = aux_kind(act, dtype);
     g.aux = g.auxk == AUX_NONE ? nullptr : aux;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == VAE_T_F32) return dense_forward_t<float>(g, workspace, s);
@@ -1007,18 +1010,18 @@ extern "C" int vae_dense_forward(const void* x, int64_t ldx, const void* w, int6
 }
 
 extern "C" int64_t vae_dense_forward_workspace_floats(int64_t M, int64_t N, int64_t K, int dtype) {
-    if (M < 1 || N < 1 || K < 1 || vae_type_size(dtype) == 0 || dense_few(M, K, vae_type_size(dtype))) return 0;
+    if (dense_check("dense_forward_workspace_floats", M, N, K, VAE_ACT_NONE, dtype) != VAE_OK || M == 0 || dense_few(M, K, vae_type_size(dtype))) return 0;
     const int es = vae_type_size(dtype);
     return forward_split(M, N, K, es) + (forward_pads(M, N, K, es) ? (M + N) * pad8(K) / 2 : 0);
 }
 
 extern "C" int64_t vae_dense_workspace_floats(int64_t M, int64_t N, int64_t K, int act, int dtype) {
-    if (M < 1 || N < 1 || K < 1 || vae_type_size(dtype) == 0) return 0;
+    if (dense_check("dense_workspace_floats", M, N, K, act, dtype) != VAE_OK || M == 0) return 0;
     return dense_ws(M, N, K, dtype, act).total;
 }
 
 extern "C" int vae_dense_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* aux,
-                                  void* dx, void* dw, void* db, float* workspace, int M, int N, int K, int act, float slope, int dtype,
+                                  void* dx, void* dw, void* db, float* workspace, int64_t M, int64_t N, int64_t K, int act, float slope, int dtype,
                                   vae_stream_t stream) {
     if (int rc = dense_check("dense_backward", M, N, K, act, dtype)) return rc;
     if (M == 0) VAE_FAIL(VAE_EINVAL, "dense_backward: no rows");
@@ -1029,7 +1032,7 @@ extern "C" int vae_dense_backward(const void* dy, int64_t lddy, const void* x, i
     if (N == 1) ldw = K;
     hipStream_t s = (hipStream_t)stream;
 #define VAE_DENSE(T) \
-    return dense_backward_t<T>((const T*)dy, lddy, (const T*)x, ldx, (const T*)w, ldw, aux, (T*)dx, (T*)dw, (T*)db, workspace, M, N, K, act, slope, dtype, s)
+    return dense_backward_t<T>((const T*)dy, lddy, (const T*)x, ldx, (const T*)w, ldw, aux, (T*)dx, (T*)dw, (T*)db, workspace, (int)M, (int)N, (int)K, act, slope, dtype, s)
     if (dtype == VAE_T_F32) VAE_DENSE(float);
     if (dtype == VAE_T_BF16) VAE_DENSE(bf16_t);
     VAE_DENSE(f16_t);

@@ -469,6 +469,7 @@ GsPlan gs_plan(int B, int T, int D, int esize, bool fwd) {
 
 template <typename T, int V, int W, bool FWD>
 int gs_launch(const GsArgs& a) {
+    VAE_FITS(FWD ? "gscan_fwd_k" : "gscan_bwd_k", gs_columns(a.B, a.D, V), W * 64);
     const dim3 grid((unsigned)gs_columns(a.B, a.D, V), a.parts);
     if constexpr (W == 16) {
         if (a.parts > 1) {
@@ -506,36 +507,39 @@ int gs_run(GsArgs& a) {
     VAE_FAIL(VAE_EINVAL, "gated_scan: no launch for V = %d, W = %d", p.V, p.W);
 }
 
-int gs_check(const char* what, int B, int T, int D, int dtype) {
+// (T: a tile may reach 2^16 steps past the last)
+bool gs_sizes(int64_t B, int64_t T, int64_t D) {
+    return B >= 0 && T >= 1 && D >= 1 && T <= 0x7fff0000 && B <= 0x7fffffff && D <= 0x7fffffff && B * D <= 0x7fffffff;
+}
+int gs_check(const char* what, int64_t B, int64_t T, int64_t D, int dtype) {
     if (vae_type_size(dtype) == 0) VAE_FAIL(VAE_EINVAL, "%s: type %d (f32, bf16 or f16)", what, dtype);
-    if (B < 0 || T < 1 || D < 1 || T > 0x7fff0000 || (int64_t)B * D > 0x7fffffff)
-        VAE_FAIL(VAE_EINVAL, "%s: %d sequences of %d steps of %d features", what, B, T, D);
+    if (!gs_sizes(B, T, D)) VAE_FAIL(VAE_EINVAL, "%s: %lld sequences of %lld steps of %lld features", what, (long long)B, (long long)T, (long long)D);
     return VAE_OK;
 }
 
 }  // namespace
 
-extern "C" int64_t vae_gated_scan_kept_floats(int B, int T, int D) {
-    if (B < 1 || T <= GS_TILE || D < 1) return 0;  // (a single tile starts from h0)
-    return ceil_div64(T, GS_TILE) * B * (int64_t)D;
+extern "C" int64_t vae_gated_scan_kept_floats(int64_t B, int64_t T, int64_t D) {
+    if (!gs_sizes(B, T, D) || T <= GS_TILE) return 0;  // (a single tile starts from h0)
+    return ceil_div64(T, GS_TILE) * B * D;
 }
 
-extern "C" int64_t vae_gated_scan_workspace_floats(int B, int T, int D, int dtype) {
-    if (B < 1 || T < 1 || D < 1 || vae_type_size(dtype) == 0) return 0;
-    const int f = gs_plan(B, T, D, vae_type_size(dtype), true).parts, b = gs_plan(B, T, D, vae_type_size(dtype), false).parts;
+extern "C" int64_t vae_gated_scan_workspace_floats(int64_t B, int64_t T, int64_t D, int dtype) {
+    if (!gs_sizes(B, T, D) || B == 0 || vae_type_size(dtype) == 0) return 0;
+    const int f = gs_plan((int)B, (int)T, (int)D, vae_type_size(dtype), true).parts, b = gs_plan((int)B, (int)T, (int)D, vae_type_size(dtype), false).parts;
     const int p = f > b ? f : b;  // (one size for both passes)
     return p > 1 ? 2 * (int64_t)p * B * D : 0;
 }
 
 extern "C" int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st,
                                       const float* h0, const int32_t* lengths, void* y, float* h_last, float* kept, float* workspace,
-                                      int B, int T, int D, int dtype, vae_stream_t stream) {
+                                      int64_t B, int64_t T, int64_t D, int dtype, vae_stream_t stream) {
     if (int rc = gs_check("gated_scan_forward", B, T, D, dtype)) return rc;
     if (B == 0) return VAE_OK;
     GsArgs a = {};
     if (x == nullptr || gate == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "gated_scan_forward: null buffer");
     a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st, a.h0 = h0, a.lengths = lengths, a.y = y, a.hl = h_last;
-    a.kept = T > GS_TILE ? kept : nullptr, a.maps = workspace, a.B = B, a.T = T, a.D = D, a.s = (hipStream_t)stream;
+    a.kept = T > GS_TILE ? kept : nullptr, a.maps = workspace, a.B = (int)B, a.T = (int)T, a.D = (int)D, a.s = (hipStream_t)stream;
     if (dtype == VAE_T_F32) return gs_run<float, true>(a);
     return dtype == VAE_T_BF16 ? gs_run<bf16_t, true>(a) : gs_run<f16_t, true>(a);
 }
@@ -543,7 +547,7 @@ extern "C" int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st,
 extern "C" int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy_st, const float* dh_last, const void* x, int64_t x_sb,
                                        int64_t x_st, const void* gate, int64_t g_sb, int64_t g_st, const float* h0,
                                        const int32_t* lengths, const float* kept, void* dx, void* dgate, float* dh0, float* workspace,
-                                       int B, int T, int D, int dtype, vae_stream_t stream) {
+                                       int64_t B, int64_t T, int64_t D, int dtype, vae_stream_t stream) {
     if (int rc = gs_check("gated_scan_backward", B, T, D, dtype)) return rc;
     if (B == 0) return VAE_OK;
     GsArgs a = {};
@@ -551,7 +555,7 @@ extern "C" int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy
         VAE_FAIL(VAE_EINVAL, "gated_scan_backward: null buffer");
     a.dy = dy, a.dyb = dy_sb, a.dyt = dy_st, a.dhl = dh_last, a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st;
     a.h0 = h0, a.lengths = lengths, a.kept = const_cast<float*>(kept), a.dx = dx, a.dg = dgate, a.dh0 = dh0, a.maps = workspace;
-    a.B = B, a.T = T, a.D = D, a.s = (hipStream_t)stream;
+    a.B = (int)B, a.T = (int)T, a.D = (int)D, a.s = (hipStream_t)stream;
     if (dtype == VAE_T_F32) return gs_run<float, false>(a);
     return dtype == VAE_T_BF16 ? gs_run<bf16_t, false>(a) : gs_run<f16_t, false>(a);
 }

@@ -16,7 +16,7 @@ namespace {
 
 // Workgroups of the backward launch = rows of partial sums: their bytes stay small beside the tensors'.
 constexpr int NORM_MAX_PARTS = 1024;
-int64_t norm_parts_cap(int C) {
+int64_t norm_parts_cap(int64_t C) {
     const int64_t n = ((int64_t)1 << 21) / C;
     return n < 256 ? 256 : n > NORM_MAX_PARTS ? NORM_MAX_PARTS : n;
 }
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_k(const T* dy, int64_t ldd
 template <typename T>
 __global__ __launch_bounds__(256) void norm_cols_long_k(const T* dy, int64_t lddy, const T* x, int64_t ldx, const float* mean_in,
                                                         const float* rstd_in, float* part, int64_t rows, int C) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= C) return;
     float dw = 0.f, db = 0.f;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
@@ -431,6 +431,7 @@ int norm_forward_t(const NormArgs& a) {
         if (a.C <= 12288) return fwd_inst<T, TW, 1024, 3>(a);
         if (a.C <= 16384) return fwd_inst<T, TW, 1024, 4>(a);
     }
+    VAE_FITS("norm_fwd_long_k", a.rows, 1024);
     norm_fwd_long_k<T, TW><<<dim3((unsigned)a.rows), dim3(1024), 0, a.s>>>((const T*)a.x, a.ldx, (const TW*)a.w, (const TW*)a.b, (T*)a.y,
                                                                            a.ldy, a.mean, a.rstd, a.C, a.eps);
     VAE_LAUNCH_CHECK("norm_fwd_long_k");
@@ -459,6 +460,7 @@ int norm_backward_t(const NormArgs& a) {
         if (a.C <= 12288) return bwd_inst<T, TW, 1024, 3, false>(a);
     }
     if (a.dx != nullptr) {
+        VAE_FITS("norm_bwd_long_k", a.rows, 1024);
         norm_bwd_long_k<T, TW><<<dim3((unsigned)a.rows), dim3(1024), 0, a.s>>>((const T*)a.dy, a.lddy, (const T*)a.x, a.ldx, (const TW*)a.w,
                                                                                a.cmean, a.crstd, (T*)a.dx, a.lddx, a.C);
         VAE_LAUNCH_CHECK("norm_bwd_long_k");
@@ -485,43 +487,44 @@ int norm_dispatch(const NormArgs& a, int dtype, int wtype) {
     return VAE_EINVAL;
 }
 
-int norm_check(const char* what, int64_t rows, int C, int dtype, int wtype) {
+int norm_check(const char* what, int64_t rows, int64_t C, int dtype, int wtype) {
     if (vae_type_size(dtype) == 0 || (wtype != VAE_T_F32 && wtype != dtype))
         VAE_FAIL(VAE_EINVAL, "%s: type %d with parameters of type %d (f32, bf16 or f16; parameters f32 or the input's type)", what, dtype, wtype);
-    if (C < 1 || rows < 0 || rows > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "%s: %lld rows of %d", what, (long long)rows, C);
+    if (C < 1 || C > 0x7fffffff || rows < 0 || rows > 0x7fffffff) VAE_FAIL(VAE_EINVAL, "%s: %lld rows of %lld", what, (long long)rows, (long long)C);
     return VAE_OK;
 }
 
 }  // namespace
 
 extern "C" int vae_layer_norm_forward(const void* x, int64_t ldx, const void* w, const void* b, void* y, int64_t ldy, float* mean,
-                                      float* rstd, int64_t rows, int C, float eps, int dtype, int wtype, vae_stream_t stream) {
+                                      float* rstd, int64_t rows, int64_t C, float eps, int dtype, int wtype, vae_stream_t stream) {
     if (int rc = norm_check("layer_norm_forward", rows, C, dtype, wtype)) return rc;
     if (rows == 0) return VAE_OK;
     if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) VAE_FAIL(VAE_EINVAL, "layer_norm_forward: null buffer");
-    if (rows > 1 && (ldx < C || ldy < C)) VAE_FAIL(VAE_EINVAL, "layer_norm_forward: row strides %lld, %lld below %d", (long long)ldx, (long long)ldy, C);
+    if (rows > 1 && (ldx < C || ldy < C)) VAE_FAIL(VAE_EINVAL, "layer_norm_forward: row strides %lld, %lld below %lld", (long long)ldx, (long long)ldy, (long long)C);
     NormArgs a = {};
-    a.x = x, a.ldx = ldx, a.w = w, a.b = b, a.y = y, a.ldy = ldy, a.mean = mean, a.rstd = rstd, a.rows = rows, a.C = C, a.eps = eps;
+    a.x = x, a.ldx = ldx, a.w = w, a.b = b, a.y = y, a.ldy = ldy, a.mean = mean, a.rstd = rstd, a.rows = rows, a.C = (int)C, a.eps = eps;
     a.s = (hipStream_t)stream;
     return norm_dispatch<true>(a, dtype, wtype);
 }
 
-extern "C" int64_t vae_layer_norm_workspace_floats(int64_t rows, int C) {
-    if (rows < 1 || C < 1) return 0;
-    return 2 * (int64_t)C * (rows < norm_parts_cap(C) ? rows : norm_parts_cap(C));
+extern "C" int64_t vae_layer_norm_workspace_floats(int64_t rows, int64_t C) {
+    if (rows < 1 || C < 1 || C > 0x7fffffff) return 0;
+    return 2 * C * (rows < norm_parts_cap(C) ? rows : norm_parts_cap(C));
 }
 
 extern "C" int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
                                        const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* workspace, int64_t rows,
-                                       int C, int dtype, int wtype, vae_stream_t stream) {
+                                       int64_t C, int dtype, int wtype, vae_stream_t stream) {
     if (int rc = norm_check("layer_norm_backward", rows, C, dtype, wtype)) return rc;
     const bool cols = dw != nullptr || db != nullptr;
     if (rows > 0 && (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (cols && workspace == nullptr)))
         VAE_FAIL(VAE_EINVAL, "layer_norm_backward: null buffer");
-    if (rows > 1 && (ldx < C || lddy < C || (dx != nullptr && lddx < C))) VAE_FAIL(VAE_EINVAL, "layer_norm_backward: a row stride below %d", C);
+    if (rows > 1 && (ldx < C || lddy < C || (dx != nullptr && lddx < C))) VAE_FAIL(VAE_EINVAL, "layer_norm_backward: a row stride below %lld", (long long)C);
+    if (cols) VAE_FITS("part_cols_k", ceil_div64(2 * C, 64), 1024);
     NormArgs a = {};
     a.dy = dy, a.lddy = lddy, a.x = x, a.ldx = ldx, a.w = w, a.cmean = mean, a.crstd = rstd, a.dx = dx, a.lddx = lddx, a.dw = dw, a.db = db;
-    a.part = workspace, a.rows = rows, a.C = C, a.s = (hipStream_t)stream;
+    a.part = workspace, a.rows = rows, a.C = (int)C, a.s = (hipStream_t)stream;
     if (rows == 0) {  // sums over nothing
         if (!cols) return VAE_OK;
         return wtype == VAE_T_F32 ? finish_parts<float>(a, 0) : dtype == VAE_T_BF16 ? finish_parts<bf16_t>(a, 0) : finish_parts<f16_t>(a, 0);

@@ -8,6 +8,14 @@ typedef _Float16 f16_t;
 
 static inline int vae_type_size(int t) { return t == VAE_T_F32 ? 4 : (t == VAE_T_BF16 || t == VAE_T_F16) ? 2 : 0; }
 
+// A launch holds fewer than 2^32 threads; one of more is refused on the host.
+#define VAE_FITS(name, blocks, threads)                                                                                            \
+    do {                                                                                                                           \
+        const int64_t b_ = (blocks);                                                                                               \
+        if (b_ > 0xffffffffll / (threads))                                                                                         \
+            VAE_FAIL(VAE_EINVAL, "%s: %lld workgroups of %d threads, more than a launch holds", name, (long long)b_, (int)(threads)); \
+    } while (0)
+
 // N elements that start on any multiple of the element's size: gfx950's global loads and stores take such addresses, so
 // rows of odd length move in 16-byte pieces like aligned ones.
 template <typename T, int N>
