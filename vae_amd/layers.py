@@ -5,11 +5,12 @@ window as a row: a module built from them trains through `vae_amd.train.train` (
 Each is one launch forward, or two or three where sums are split or ragged rows laid out anew, and differentiable once.
 Tensors are fp32, bf16 or fp16 on an MI355X; sums, statistics and states are fp32 (include/vae_amd.h, vae_layer_norm_* /
 vae_dense_* / vae_gated_scan_*).  Calls run on the current stream of the tensors' device, allocate through torch's allocator
-and can be captured in a graph.  Before a backward pass is captured, drop the eager graphs (losses, outputs) of the same
-leaves: torch ties a leaf's gradient node to the stream of the first graph that it was in and would wait for that stream inside
-the capture, which ends the process.
+and can be captured in a graph.  Forward-mode duals, and calls under torch.jit.trace or make_fx, are refused.  Before a backward
+pass is captured, drop the eager graphs (losses, outputs) of the same leaves: torch ties a leaf's gradient node to the stream of
+the first graph that it was in and would wait for that stream inside the capture, which ends the process.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -85,12 +86,22 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise L.VaeAmdError("vae_amd.layers: no forward-mode derivative of a backward pass")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
 
-def _needs_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _through_function(what, *ts):
+    """Does the call go through its autograd function: where a gradient is asked for, and where forward-mode duals may be about (the
+    function refuses them).  The kernels write through pointers: of a bare call torch sees the empty result alone, so a dual would lose
+    its tangent and a trace keep the allocation.  Tracing is refused with gradients too: a replay skips the checks of types and sizes."""
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise L.VaeAmdError(f"{what}: torch.jit.trace and make_fx cannot record this call")
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts))
 
 
 # ------------------------------------------------------------------------------------------------ layer norm
@@ -154,7 +165,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         _same("layer_norm", bias, "bias", shape, kinds if weight is None else (weight.dtype,), device)
         if not bias.is_contiguous():
             bias = bias.contiguous()
-    if _needs_grad(x, weight, bias):
+    if _through_function("layer_norm", x, weight, bias):
         return _NormFn.apply(x, weight, bias, float(eps), device, code)
     return _norm_forward(x, weight, bias, float(eps), device, code, False)[0]
 
@@ -228,7 +239,7 @@ def linear(x, weight, bias=None, act="none", slope=0.0, residual=None):
             bias = bias.contiguous()
     if residual is not None:
         _same("linear", residual, "residual", x.shape[:-1] + shape[:1], kinds, device)
-    if _needs_grad(x, weight, bias, residual):
+    if _through_function("linear", x, weight, bias, residual):
         return _LinearFn.apply(x, weight, bias, residual, _ACTS[act], float(slope), device, code)
     return _linear_forward(x, weight, bias, _ACTS[act], float(slope), residual, device, code, False)[0]
 
@@ -316,6 +327,6 @@ def gated_scan(x, gate, h0=None, lengths=None):
     if B == 0 or T == 0 or D == 0:  # no step: the state stays
         h = h0 if h0 is not None else torch.zeros(B, D, device=device)
         return x * gate, h.clone()
-    if _needs_grad(x, gate, h0):
+    if _through_function("gated_scan", x, gate, h0):
         return _ScanFn.apply(x, gate, h0, lengths, device, code)
     return _scan_forward(x, gate, h0, lengths, device, code, False)[:2]
