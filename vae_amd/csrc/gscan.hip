@@ -372,7 +372,7 @@ __global__ __launch_bounds__(W * 64) void gscan_bwd_k(const GsArgs a) {
                     const float dh = q[v] + ds[s][v];
                     q[v] = f[s][v] * dh;
                     ox[v] = i[s][v] * dh;
-                    og[v] = q[v] * xs[s][v] * i[s][v];
+                    og[v] = q[v] * i[s][v] * xs[s][v];  // (f i first: where it is 0, the states' difference may be anything)
                 }
                 if (stores_full) {
                     if (a.dx != nullptr) store_part<T, V>(xp, ox, V);

@@ -86,8 +86,8 @@ __device__ __forceinline__ void store_part(T* p, const float (&r)[N], int64_t le
     }
 }
 
-// exp(x) with a relative error of about 1e-7 over the whole range: 2^t of t = x log2(e), corrected by what rounding t lost
-// (without the correction |t| 2^-24 enters the result: 1e-6 at |x| = 10).
+// exp(x), |x| <= 2^126, with a relative error of about 1e-7: 2^t of t = x log2(e), corrected by what rounding t lost (without the
+// correction |t| 2^-24 enters the result: 1e-6 at |x| = 10).  Results below 2^-126 are 0.  (Where t is infinite the correction is a NaN.)
 __device__ __forceinline__ float exp_acc(float x) {
     const float t = x * 1.44269504f;
     const float lost = fmaf(x, 1.44269504f, -t) + x * 1.9259629e-8f;
@@ -98,8 +98,8 @@ __device__ __forceinline__ float exp_acc(float x) {
 // ... and one of |x| 2^-24, in two instructions, for results that are rounded to 16 bits
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
-// f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1); infinite gates give
-// 0 and 1, a NaN passes.  FAST, for 16-bit tensors: exp may be off by |g| 2^-24; f then is by (1 - f) of that, so over the
+// f = sigmoid(g) and i = sigmoid(-g), each to full relative precision (1 - f would lose i where f is near 1) as long as it is 2^-126 or
+// more, and 0 below; infinite gates give 0 and 1, a NaN passes.  FAST, for 16-bit tensors: exp may be off by |g| 2^-24; f then is by (1 - f) of that, so over the
 // 1 / (1 - f) steps that a recurrence remembers it adds up to no more.
 template <bool FAST = false>
 __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
@@ -108,11 +108,10 @@ __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
         f = __builtin_amdgcn_rcpf(1.f + e);
         i = e > 1e30f ? 1.f : e * f;  // (where e is infinite)
     } else {
-        g = g > 87.f ? 87.f : g;  // (keeps exp_acc finite)
-        g = g < -87.f ? -87.f : g;
-        const float e = exp_acc(-g);
-        f = __builtin_amdgcn_rcpf(1.f + e);  // (one unit in the last place)
-        i = e * f;
+        const float m = fabsf(g) > 128.f ? 128.f : fabsf(g), e = exp_acc(-m);  // (of the smaller one: it goes down to 0)
+        const float more = __builtin_amdgcn_rcpf(1.f + e), less = e * more;    // (one unit in the last place)
+        f = g < 0.f ? less : more;
+        i = g < 0.f ? more : less;
     }
 }
 
