@@ -1,11 +1,64 @@
-"""Values of the sequence-block operators far out: gates from 200 to infinity on either side."""
+"""Values of the sequence-block operators far out: activations and gates from 20 to infinity on either side.
+
+Below 2^-126 an exponential may be 0: its value times a factor of at most 128 is then off by 2^-119 at most."""
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
+U = 2.0 ** -24
+LOST = 2.0 ** -119
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 IDS = ["f32", "bf16", "f16"]
+FAR = [20.0, 50.0, 87.0, 87.5, 88.0, 88.5, 90.0, 104.0, 200.0, 1e4, 6e4, 1e19, 3e19, 1e20, 1e30, 1e35, 3e38, float("inf")]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def smallest(dtype):
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+
+
+def act_limits(p, act, slope):
+    """act and act' in 64 bits; at -inf (and +inf) their limits."""
+    if act == "leaky":
+        return torch.where(p > 0, p, 0.0 * p.sign() if slope == 0 else slope * p), torch.where(p > 0, 1.0, slope).double()
+    q = p.clamp(-1e300, 1e300)  # (a limit: what multiplies the vanishing factor is finite)
+    s, c = torch.sigmoid(q), torch.special.ndtr(q)
+    if act == "sigmoid":
+        return s, s * torch.sigmoid(-q)
+    if act == "silu":
+        return torch.where(p == float("inf"), p, q * s), s * (1 + q * torch.sigmoid(-q))
+    return torch.where(p == float("inf"), p, q * c), c + q * torch.exp(-(q.clamp(-1e3, 1e3)) ** 2 / 2) * 0.3989422804014327
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("act,slope", [("leaky", 0.0), ("leaky", 0.25), ("sigmoid", 0.0), ("gelu", 0.0), ("silu", 0.0)])
+@pytest.mark.parametrize("rows", [40, 700])
+def test_activations_far_out(act, slope, dtype, rows):
+    """Through the form of few rows and through tiles.  One product a value: p is the input itself.  A sigmoid's exponent loses |p| U for
+    16-bit results; act' sees p as it is kept (2^-11 of it for bf16), which moves it by |p act''| 2^-11, |act''| <= 2 |act'| out here."""
+    from vae_amd import layers
+    x = torch.tensor(FAR + [-v for v in FAR] + [float("nan")], dtype=torch.float64).to(dtype).cuda()
+    x = x.repeat(-(-rows // len(x)))[:rows, None].contiguous().requires_grad_()
+    y = layers.linear(x, torch.ones(1, 1, dtype=dtype, device="cuda"), act=act, slope=slope)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    p = x.detach().double()
+    v, d = act_limits(p, act, slope)
+    nan = p.isnan()
+    assert (y.isnan() == nan).all(), p[y.isnan() != nan]
+    assert not dx[~nan].isnan().any(), p[dx.isnan() & ~nan]
+    fine = ~nan & v.isfinite()
+    assert (y.double()[~nan & ~fine] == v[~nan & ~fine]).all()
+    near = p.abs().clamp(max=128)
+    tol = (half(dtype) + 32 * U + 2 * near * U) * v.abs() + LOST + smallest(dtype)
+    assert ((y.double() - v).abs() <= tol)[fine].all(), p[fine & ~((y.double() - v).abs() <= tol)]
+    tol = (half(dtype) + 32 * U + near * 2.0 ** -9) * d.abs() + LOST + smallest(dtype)
+    if act == "leaky":
+        tol = half(dtype) * d.abs()
+    assert ((dx.double() - d).abs() <= tol)[~nan].all(), p[~nan & ~((dx.double() - d).abs() <= tol)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

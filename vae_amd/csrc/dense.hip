@@ -31,10 +31,11 @@ inline int aux_kind(int act, int dtype) {
 }
 
 // Normal distribution function and exp(-p^2/2): erfc by Abramowitz & Stegun 7.1.26, (a1 t + .. + a5 t^5) exp(-x^2) with
-// t = 1 / (1 + 0.3275911 x), x = |p| / sqrt 2, off by at most 1.5e-7 (the function half of that); no branches.
+// t = 1 / (1 + 0.3275911 x), x = |p| / sqrt 2, off by at most 1.5e-7 (the function half of that); no branches.  0 and 1 far out.
 template <bool FAST>
 __device__ __forceinline__ float normal_cdf(float p, float& e) {
-    const float x = fabsf(p) * 0.70710678f;
+    float x = fabsf(p) * 0.70710678f;
+    if (!FAST) x = x > 12.f ? 12.f : x;  // (keeps exp_acc finite; the result is 0 by then)
     e = FAST ? exp_fast(-x * x) : exp_acc(-x * x);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
     float u = fmaf(t, 1.061405429f, -1.453152027f);
@@ -44,14 +45,16 @@ __device__ __forceinline__ float normal_cdf(float p, float& e) {
     return p < 0.f ? u : 1.f - u;
 }
 
-// act and act' of 8 values: the switch stands outside the loop over them.  FAST: the results are rounded to 16 bits.
+// act and act' of 8 values: the switch stands outside the loop over them.  FAST: the results are rounded to 16 bits.  Minus infinity has
+// the limit of its activation (0 times infinity would be a NaN; a NaN passes).
+constexpr float ACT_LOWEST = -3.4028235e38f;
 template <bool FAST>
 __device__ __forceinline__ void dense_act8(float (&v)[8], int act, float slope) {
     float f, i;
     switch (act) {
         case VAE_ACT_LEAKY:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] > 0.f ? v[e] : v[e] * slope;
+            for (int e = 0; e < 8; ++e) v[e] = v[e] > 0.f ? v[e] : slope != 0.f ? v[e] * slope : v[e] < 0.f ? 0.f : v[e];
             break;
         case VAE_ACT_SIGMOID:
 #pragma unroll
@@ -59,11 +62,11 @@ __device__ __forceinline__ void dense_act8(float (&v)[8], int act, float slope) 
             break;
         case VAE_ACT_GELU:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= normal_cdf<FAST>(v[e], f);
+            for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], ACT_LOWEST) * normal_cdf<FAST>(v[e], f);
             break;
         case VAE_ACT_SILU:
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate_pair<FAST>(v[e], f, i), v[e] *= f;
+            for (int e = 0; e < 8; ++e) gate_pair<FAST>(v[e], f, i), v[e] = fmaxf(v[e], ACT_LOWEST) * f;
             break;
     }
 }
