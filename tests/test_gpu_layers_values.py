@@ -1,4 +1,4 @@
-"""Values of the sequence-block operators far out: activations and gates from 20 to infinity on either side.
+"""Values of the sequence-block operators far out: activations and gates from 20 to infinity on either side, GELU's tail.
 
 Below 2^-126 an exponential may be 0: its value times a factor of at most 128 is then off by 2^-119 at most."""
 import pytest
@@ -90,3 +90,33 @@ def test_gates_far_out_are_0_and_1(gate, dtype, t):
     assert torch.allclose(h, held[:, -1], rtol=0, atol=0, equal_nan=True)
     dx, dg = torch.autograd.grad([y, h], [big, keep], [dy, dh])
     assert (dx == 0).all() and (dg[~lost] == 0).all() and dg[lost].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 3000])
+def test_gelu_to_its_tail(dtype, rows):
+    """GELU and its derivative relative to their values, down to 1e-36.  fp32: exp and its correction lose 3 U, 1 / (1 + c |p|) 3 U, eight steps of
+    the polynomial 3 U, the products 3 U, its fit 0.2 U: 13 U, and a half step of the result.  For 16-bit results exp loses p^2 U more,
+    170 U at p = -13; their derivative sees p as it is kept (2^-11 of it for bf16, |act''| <= 0.8 + p^2 phi)."""
+    from vae_amd import layers
+    x = torch.linspace(-13, 13, 3000, dtype=torch.float64).to(dtype).cuda()
+    w = torch.ones(1, 1, dtype=dtype, device="cuda")
+    if rows == 1:  # (the form of one row: a product of one value each, the weights carry the points)
+        got = layers.linear(torch.ones(1, 1, dtype=dtype, device="cuda"), x[:, None].contiguous(), act="gelu")[0]
+        dx = None
+    else:
+        xg = x[:, None].clone().requires_grad_()
+        y = layers.linear(xg, w, act="gelu")
+        got = y.detach()[:, 0]
+        dx = torch.autograd.grad(y, xg, torch.ones_like(y))[0][:, 0]
+    p = x.double()  # (torch.special.ndtr is (1 + erf) / 2, which loses the tail)
+    cdf, pdf = 0.5 * torch.special.erfc(-p * 0.5 ** 0.5), torch.exp(-p * p / 2) * 0.3989422804014327
+    v = p * cdf
+    off = 13 * U if dtype == torch.float32 else (13 + p * p) * U
+    err = (got.double() - v).abs()
+    assert (err <= (half(dtype) + off) * v.abs() + LOST + smallest(dtype)).all(), float((err / v.abs().clamp(min=1e-30)).max())
+    if dx is not None:
+        d = cdf + p * pdf
+        kept = 2.0 ** -11 * p.abs() * (2 * pdf + p * p * pdf) if dtype == torch.bfloat16 else 0.0
+        err = (dx.double() - d).abs()
+        assert (err <= half(dtype) * d.abs() + (off + 2 * U) * (cdf + p.abs() * pdf) + kept + LOST + smallest(dtype)).all(), float(err.max())
