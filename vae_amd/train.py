@@ -303,8 +303,7 @@ def train(model, train_loader, criterion, optimizer, device, epoch):
             x_rec, mu, logvar = model(data)
             target = data[:, :, 0] if data.dim() == 3 else data
             loss = criterion(x_rec, target, mu, logvar)
-            with torch.autograd.set_multithreading_enabled(False):  # one GPU a process: a thread of its own only costs the hand-over
-                loss.backward()
+            loss.backward()
             optimizer.step()
             total_dev = loss.detach().clone().reshape(1) if total_dev is None else total_dev.add_(loss.detach())
         if batch_idx % 100 == 0:
