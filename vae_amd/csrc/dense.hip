@@ -418,9 +418,9 @@ __global__ __launch_bounds__(256) void gemm_pair_k(const GemmArgs dw, int dw_til
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t lds_addr, uint32_t voff) {
-    // no register is written and the addresses are read when the instruction issues; the caller waits (vmcnt) before the
-    // barrier behind which the tile is read
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_addr), "v"(voff), "s"(rsrc));
+    // no register is written (the LDS address goes in as m0: the compiler puts it there) and the addresses are read when the instruction
+    // issues; the caller waits (vmcnt) before the barrier behind which the tile is read
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(lds_addr), "v"(voff), "s"(rsrc));
 }
 
 constexpr int HB = 64;  // bytes of k in a half tile
