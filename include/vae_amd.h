@@ -328,9 +328,10 @@ int vae_window_gather(const float* series, int C, int64_t T, int L, const int64_
  * window as a row.  No counterpart in the reference, whose recurrent models are torch LSTMs (Encoders.py:110-147).
  * dtype = VAE_T_* of the tensors; strides are in elements, rows are contiguous (any alignment, any stride >= the row).  All
  * sums, statistics and states are fp32.  Workspaces are caller-owned, sized by the *_floats / *_bytes queries (host-only), need no
- * clearing and hold nothing between calls; calls that may overlap need a workspace each.  Results are bit-identical from run to
- * run (no float atomics).  Sizes are 64-bit so that what is too large is seen and refused: rows and columns of a norm up to 2^31 - 1,
- * M, N, K of a linear layer up to 2^30 - 1, T up to 2^31 - 2^16, B D up to 2^31 - 1, and no launch of 2^32 threads.
+ * clearing and hold nothing between calls; calls that may overlap need a workspace each.  No output shares memory with an input.
+ * Results are bit-identical from run to run (no float atomics).  Sizes are 64-bit so that what is too large is seen and refused:
+ * rows and columns of a norm up to 2^31 - 1, M, N, K of a linear layer up to 2^30 - 1, T up to 2^31 - 2^16, B D up to 2^31 - 1,
+ * and no launch of 2^32 threads.
  *
  * Layer norm over rows of C: y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) with the biased variance.  w, b: type wtype
  * (VAE_T_F32 or dtype), NULL = 1 / 0.  mean, rstd (rows floats each; both or neither): what the backward pass needs.

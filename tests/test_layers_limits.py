@@ -87,3 +87,12 @@ def test_launches_of_2_to_the_32_threads():
     _refused(_dense_bwd(2 ** 30 - 1, 9, 64), "more than a launch holds")
     _refused(_scan_fwd(2 ** 30, 40, 1), "more than a launch holds")
     _refused(_scan_bwd(2 ** 30, 40, 1), "more than a launch holds")
+
+
+def test_a_state_is_not_advanced_in_place():
+    """The last lanes of a sequence share features with their neighbours: with h_last in h0's memory one could read what the other wrote."""
+    from vae_amd import _lib as L
+    lib, n = L.lib(), 3 * 7
+    for at in (P, P + 4, P + 4 * (n - 1), P - 4 * (n - 1)):
+        _refused(lib.vae_gated_scan_forward(P, 7, 7, P, 7, 7, P, None, P, at, None, None, 3, 1, 7, 0, None), "h_last")
+        _refused(lib.vae_gated_scan_backward(P, 7, 7, P, P, 7, 7, P, 7, 7, None, None, None, P, P, at, None, 3, 1, 7, 0, None), "dh0")

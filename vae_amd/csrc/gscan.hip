@@ -517,6 +517,12 @@ int gs_check(const char* what, int64_t B, int64_t T, int64_t D, int dtype) {
     return VAE_OK;
 }
 
+// Do two arrays of B D floats share memory?  (A state advanced in place: lanes that share features could read what their neighbours wrote.)
+bool gs_overlap(const float* p, const float* q, int64_t n) {
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return p != nullptr && q != nullptr && (a < b ? b - a : a - b) < (uintptr_t)n * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" int64_t vae_gated_scan_kept_floats(int64_t B, int64_t T, int64_t D) {
@@ -538,6 +544,7 @@ extern "C" int vae_gated_scan_forward(const void* x, int64_t x_sb, int64_t x_st,
     if (B == 0) return VAE_OK;
     GsArgs a = {};
     if (x == nullptr || gate == nullptr || y == nullptr) VAE_FAIL(VAE_EINVAL, "gated_scan_forward: null buffer");
+    if (gs_overlap(h0, h_last, B * D)) VAE_FAIL(VAE_EINVAL, "gated_scan_forward: h_last shares memory with h0");
     a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st, a.h0 = h0, a.lengths = lengths, a.y = y, a.hl = h_last;
     a.kept = T > GS_TILE ? kept : nullptr, a.maps = workspace, a.B = (int)B, a.T = (int)T, a.D = (int)D, a.s = (hipStream_t)stream;
     if (dtype == VAE_T_F32) return gs_run<float, true>(a);
@@ -553,6 +560,7 @@ extern "C" int vae_gated_scan_backward(const void* dy, int64_t dy_sb, int64_t dy
     GsArgs a = {};
     if (x == nullptr || gate == nullptr || (T > GS_TILE && kept == nullptr))
         VAE_FAIL(VAE_EINVAL, "gated_scan_backward: null buffer");
+    if (gs_overlap(dh_last, dh0, B * D)) VAE_FAIL(VAE_EINVAL, "gated_scan_backward: dh0 shares memory with dh_last");
     a.dy = dy, a.dyb = dy_sb, a.dyt = dy_st, a.dhl = dh_last, a.x = x, a.xb = x_sb, a.xt = x_st, a.g = gate, a.gb = g_sb, a.gt = g_st;
     a.h0 = h0, a.lengths = lengths, a.kept = const_cast<float*>(kept), a.dx = dx, a.dg = dgate, a.dh0 = dh0, a.maps = workspace;
     a.B = (int)B, a.T = (int)T, a.D = (int)D, a.s = (hipStream_t)stream;
