@@ -347,7 +347,9 @@ int vae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
  * (slope: of the leaky ReLU).  aux (vae_dense_aux_bytes; NULL when no backward pass follows): what act' needs of p.  workspace
  * (vae_dense_forward_workspace_floats; NULL where that is 0): slices of products of few outputs, copies of large ragged operands.
  * Backward: dp = dy act'(p); dx = dp w (M x K, dense), dw = dp^T x (N x K, dense), db = column sums of dp; each optional.  The
- * residual's gradient is dy itself. */
+ * residual's gradient is dy itself.  Two roundings to fewer bits, for 16-bit tensors: dp is rounded to dtype before its two products (the
+ * matrix cores take their operands so; db is summed before that rounding), and p is kept for act' in fp16 where dtype is bf16 (in fp32
+ * where it is fp16 or fp32; a byte for the leaky ReLU). */
 int64_t vae_dense_aux_bytes(int64_t M, int64_t N, int act, int dtype);
 int vae_dense_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr,
                       void* y, int64_t ldy, void* aux, float* workspace, int64_t M, int64_t N, int64_t K, int act, float slope,
