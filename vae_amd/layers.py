@@ -92,14 +92,14 @@ def _once(backward):
     return run
 
 
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _modes, _PROXY = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._TorchDispatchModeKey.PROXY
 
 
 def _through_function(what, *ts):
     """Does the call go through its autograd function: where a gradient is asked for, and where forward-mode duals may be about (the
     function refuses them).  The kernels write through pointers: of a bare call torch sees the empty result alone, so a dual would lose
     its tangent and a trace keep the allocation.  Tracing is refused with gradients too: a replay skips the checks of types and sizes."""
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None):
         raise L.VaeAmdError(f"{what}: torch.jit.trace and make_fx cannot record this call")
     return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts))
 
