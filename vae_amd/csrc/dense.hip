@@ -476,10 +476,11 @@ struct Dma {
 // h + 1 are read, and the loads of h + 4 are issued into the slot of a ring of four that h has left: a load has two phases and more
 // to arrive.  One barrier a phase says that h + 2 has landed for every wave and that h + 1 has been read by every wave.  Reads and
 // loads stand between the matrix instructions, one at a time, where their issue costs nothing.
-//   16,384 x 4,096 x 4,096 bf16 (0.55 TFLOP each): forward with bias, GELU, residual and what its derivative needs 614 us, dx 465
-// (1.18 PFLOP/s), dW 403 (1.36); register-staged 128 x 128 tiles: 938, 736, 662.
-// The clock falls to 1.5 to 1.9 GHz meanwhile, so what saves waits alone gains nothing: workgroups that stay and load into their
-// next tile during the epilogue measured 634 us forward, whole 128-byte lines of k 418 against 449 for a bare forward product but
+//   16,384 x 4,096 x 4,096 bf16 (0.55 TFLOP each), in a trace of the kernels: forward with bias, GELU, residual and what its derivative
+// needs 628 us, dx 478 (1.15 PFLOP/s), dW 415 (1.33); register-staged 128 x 128 tiles: 938, 736, 662.  Of the forward pass the product and bias
+// are 470, GELU 30, the kept p 30, the residual 90: the epilogue has one wave a SIMD and the matrix cores stand still meanwhile.
+// The clock falls to 1.5 to 1.9 GHz, so in the k-loop what saves waits alone gains nothing: workgroups that stay and load into their
+// next tile during the epilogue measured 634 us forward (614 without), whole 128-byte lines of k 418 against 449 for a bare forward product but
 // registers beyond the file for dW, 32 x 32 matrix instructions 855 against 849.
 template <typename T, int BM, int BN, bool ARC, bool BRC>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_dma_k(const GemmArgs g) {

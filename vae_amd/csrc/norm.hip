@@ -7,7 +7,7 @@
 // Bound: bytes.  Groups of 4..64 lanes (several rows a wave) keep the lanes of short rows busy and sum with lane shuffles
 // alone; longer rows take a workgroup.  The backward pass keeps dw and db of the lane's own columns in registers over all rows
 // that its group visits; workgroups leave one row of partials each, which a second launch adds in a fixed order (no atomics:
-// two runs give the same bits).  65,536 x 1,024 bf16: forward 46 us (5.8 TB/s), backward 77 + 5 (4.9).
+// two runs give the same bits).  65,536 x 1,024 bf16: forward 47 us (5.8 TB/s), backward 77 + 4 (5.0).
 #include <atomic>
 
 #include "seqops.h"
@@ -456,7 +456,7 @@ int norm_backward_t(const NormArgs& a) {
     if (p <= 1024) return bwd_inst<T, TW, 1024, 1>(a);
     if (p <= 1536) return bwd_inst<T, TW, 512, 3>(a);
     if (p <= 2048) return bwd_inst<T, TW, 512, 4>(a);
-    if constexpr (sizeof(T) == 4) {  // (4 pieces a lane spill: 150 us for 2,048 x 16,384, 146 in two passes)
+    if constexpr (sizeof(T) == 4) {  // (3 pieces a lane put 20 bytes in scratch memory, 4 more: 150 us for 2,048 x 16,384, 146 in two passes)
         if (a.C <= 12288) return bwd_inst<T, TW, 1024, 3, false>(a);
     }
     if (a.dx != nullptr) {
