@@ -120,3 +120,15 @@ def test_gelu_to_its_tail(dtype, rows):
         kept = 2.0 ** -11 * p.abs() * (2 * pdf + p * p * pdf) if dtype == torch.bfloat16 else 0.0
         err = (dx.double() - d).abs()
         assert (err <= half(dtype) * d.abs() + (off + 2 * U) * (cdf + p.abs() * pdf) + kept + LOST + smallest(dtype)).all(), float(err.max())
+
+
+def test_sigmoid_to_a_unit():
+    """fp32.  exp(-|g|) = e is off by 2.2 U (2^t by a unit in the last place, its correction 0.2 U): 1 / (1 + e) by half of that at most and its
+    own rounding of U, the product e / (1 + e) by all of it and two roundings."""
+    from vae_amd import layers
+    g = torch.linspace(-30, 30, 1000001, dtype=torch.float64).float().cuda()
+    y = layers.linear(g[:, None].contiguous(), torch.ones(1, 1, device="cuda"), act="sigmoid")[:, 0]
+    want = torch.sigmoid(g.double())
+    off = (y.double() - want).abs() / want / U
+    assert off[g >= 0].max() <= 2.1, float(off[g >= 0].max())
+    assert off[g < 0].max() <= 4.2, float(off[g < 0].max())

@@ -109,7 +109,11 @@ __device__ __forceinline__ void gate_pair(float g, float& f, float& i) {
         i = e > 1e30f ? 1.f : e * f;  // (where e is infinite)
     } else {
         const float m = fabsf(g) > 128.f ? 128.f : fabsf(g), e = exp_acc(-m);  // (of the smaller one: it goes down to 0)
-        const float more = __builtin_amdgcn_rcpf(1.f + e), less = e * more;    // (one unit in the last place)
+        // 1 / (1 + e): a step of Newton's on the reciprocal, which is off by a unit in the last place, with what 1 + e lost when it was rounded
+        const float d = 1.f + e, lost = e - (d - 1.f);
+        float more = __builtin_amdgcn_rcpf(d);
+        more = fmaf(more, fmaf(-lost, more, fmaf(-d, more, 1.f)), more);
+        const float less = e * more;
         f = g < 0.f ? less : more;
         i = g < 0.f ? more : less;
     }
