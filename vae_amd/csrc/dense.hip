@@ -477,7 +477,7 @@ struct Dma {
 // to arrive.  One barrier a phase says that h + 2 has landed for every wave and that h + 1 has been read by every wave.  Reads and
 // loads stand between the matrix instructions, one at a time, where their issue costs nothing.
 //   16,384 x 4,096 x 4,096 bf16 (0.55 TFLOP each), in a trace of the kernels: forward with bias, GELU, residual and what its derivative
-// needs 628 us, dx 478 (1.15 PFLOP/s), dW 415 (1.33); register-staged 128 x 128 tiles: 938, 736, 662.  Of the forward pass the product and bias
+// needs 617 us, dx 464 (1.18 PFLOP/s), dW 398 (1.38; 628, 478 and 415 on another card); register-staged 128 x 128 tiles: 938, 736, 662.  Of the forward pass the product and bias
 // are 470, GELU 30, the kept p 30, the residual 90: the epilogue has one wave a SIMD and the matrix cores stand still meanwhile.
 // The clock falls to 1.5 to 1.9 GHz, so in the k-loop what saves waits alone gains nothing: workgroups that stay and load into their
 // next tile during the epilogue measured 634 us forward (614 without), whole 128-byte lines of k 418 against 449 for a bare forward product but

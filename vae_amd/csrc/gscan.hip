@@ -14,7 +14,7 @@
 // With few channels the time axis is also cut over workgroups (parts): a first launch leaves each part's map, the second
 // composes the maps of the parts before its own.
 // Steps at and behind a sequence's length hold the state (f = 1, i = 0) whatever lies there; y, dx, dg are 0.
-// Bound: bytes.  8 x 4,096 x 2,048 bf16, in a trace of the kernels: forward 94 us (4.3 TB/s), backward 159 (4.2); 1 x 65,521 x 512 fp32, in
+// Bound: bytes.  8 x 4,096 x 2,048 bf16, in a trace of the kernels: forward 95 us (4.2 TB/s), backward 157 (4.3); 1 x 65,521 x 512 fp32, in
 // parts: 149 and 177.  (Forward with 16 waves has 5 registers too few and keeps 24 bytes a lane in scratch memory.)
 #include "seqops.h"
 
